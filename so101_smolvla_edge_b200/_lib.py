@@ -1,4 +1,5 @@
-"""ctypes binding of libso101_b200.so (the C ABI declared in include/so101_b200.h).
+"""ctypes binding of libso101_b200.so (the C ABI declared in include/so101_b200.h and, for the text
+tower's packed attention and paged cache, include/so101_b200_text.h).
 
 The library is required: `lib()` raises if the shared object is missing or fails to load, and
 there is no other implementation to fall back to. `build.py` produces it in-tree.
@@ -14,8 +15,9 @@ from pathlib import Path
 from .build import LIB
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "so101_b200.h"
+TEXT_HEADER = HEADER.with_name("so101_b200_text.h")
 
-OK, ERR_ARG, ERR_LAUNCH, ERR_WORKSPACE, ERR_TIMEOUT, ERR_DRIVER = range(6)
+OK, ERR_ARG, ERR_LAUNCH, ERR_WORKSPACE, ERR_TIMEOUT, ERR_DRIVER, ERR_PAGES = range(7)
 BF16, F32, I8 = 0, 1, 2
 EPI_NONE, EPI_GELU, EPI_SILU_GATE = 0, 1, 2
 ERRORS = {
@@ -24,6 +26,7 @@ ERRORS = {
     ERR_WORKSPACE: "split-K workspace or tickets too small",
     ERR_TIMEOUT: "a device wait timed out",
     ERR_DRIVER: "cuTensorMapEncodeTiled unavailable",
+    ERR_PAGES: "a sequence, page or row index out of range, or too few free pages",
 }
 
 
@@ -86,6 +89,16 @@ class ExpertStep(C.Structure):
         ("act", P), ("cos_self", P), ("sin_self", P), ("cos_cross", P), ("sin_cross", P),
         ("workspace", P), ("workspace_bytes", C.c_int64)]  # fmt: skip
 
+
+class KvPages(C.Structure):
+    """`so101_kv_pages`: the paged 8-bit K/V cache's arrays and sizes."""
+
+    _fields_ = [(n, P) for n in ("k", "v", "k_scale", "v_scale", "table", "lengths", "refs", "scratch")] + [
+        (n, C.c_int) for n in ("n_layers", "n_pages", "n_kv", "page", "hd", "max_seqs", "max_pages")]  # fmt: skip
+
+
+PAGES = C.POINTER(KvPages)
+
 SIGNATURES = {
     "so101_gemm": [I, P, I64, P, I64, P, I64, I, I64, I64, I64, C.POINTER(Epilogue),
                    C.POINTER(GemmConfig), P, I64, P, I64, S],
@@ -121,12 +134,22 @@ SIGNATURES = {
     "so101_expert_step_workspace": [C.POINTER(ExpertStep), C.POINTER(C.c_int64)],
     "so101_expert_step_run": [C.POINTER(ExpertStep), S],
     "so101_expert_step_test_hooks": [I64, I],
+    "so101_attention_packed": [P, I64, P, I64, P, I64, P, I64, I64, P, I, I64, I, I, I, F, P, P, S],
+    "so101_kv_scratch": [PAGES, C.POINTER(C.c_int64)],
+    "so101_kv_append": [PAGES, I, P, I64, P, I64, I64, P, P, I, I64, P, P, S],
+    "so101_kv_read": [PAGES, I, P, P, P, I, I64, P, I64, P, I64, S],
+    "so101_attention_pages": [P, I64, P, I64, I64, PAGES, I, I, P, P, I, I64, I, F, P, P, P, I64, P, I64, S],
+    "so101_kv_reserve": [PAGES, P, P, I, S],
+    "so101_kv_free": [PAGES, P, I, S],
+    "so101_kv_fork": [PAGES, P, P, I, S],
+    "so101_kv_copy": [PAGES, P, P, I, S],
+    "so101_kv_compact": [PAGES, S],
 }  # fmt: skip
 
 
-def header_symbols() -> list[str]:
-    """Every function the C header declares."""
-    text = HEADER.read_text()
+def header_symbols(header: Path = HEADER) -> list[str]:
+    """Every function a C header declares."""
+    text = header.read_text()
     return sorted(set(re.findall(r"SO101_API\s+[\w\s\*]*?\b(so101_\w+)\s*\(", text)))
 
 

@@ -6,6 +6,14 @@
     rope_kv    kernels/rope.py:481-506        RoPE on the keys + K/V cache write
     rms_norm   kernels/norm.py:423-440        fp32 statistics, one rounding
 
+and, with no counterpart in the reference, the text tower's serving operators:
+
+    attention_packed   causal GQA over whole prompts packed end to end
+    kv_append          new keys (rotated) and values into a `pages.KvPages` cache, 8 bits
+    kv_read            cached tokens back as bf16 rows
+    attention_pages    the last tokens of each sequence over its cached ones
+    kv_reserve, kv_free, kv_fork, kv_copy, kv_compact   the cache's pages
+
 Every call goes through the C ABI of libso101_b200.so on the tensors' current CUDA stream.
 Preconditions the kernels cannot meet raise ValueError, as the reference's wrappers do.
 """
@@ -17,6 +25,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
+from .pages import KvPages
 
 DTYPE = {torch.bfloat16: L.BF16, torch.float32: L.F32, torch.int8: L.I8}
 
@@ -464,3 +473,225 @@ def set_pdl(enable: bool) -> None:
     """Launch GEMMs with programmatic dependent launch (they start streaming weights while the
     previous kernel on the stream drains)."""
     L.check(L.lib().so101_set_pdl(1 if enable else 0), "so101_set_pdl")
+
+
+_PAGES_WS: dict[tuple[torch.device, int], Workspace] = {}
+
+
+def pages_workspace(device: torch.device, stream: int) -> Workspace:
+    """The partial results of `attention_pages` on one stream (calls on several streams overlap, so
+    each has its own). It must exist before a CUDA graph is captured on the stream."""
+    ws = _PAGES_WS.get((device, stream))
+    if ws is None:
+        ws = _PAGES_WS[device, stream] = Workspace(device, nbytes=32 << 20)
+    return ws
+
+
+def _ints(dev: torch.device, **ts: torch.Tensor | None) -> None:
+    for name, t in ts.items():
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != dev):
+            raise ValueError(f"{name} must be a contiguous int32 vector on {dev}")
+
+
+def _tables(cos: torch.Tensor | None, sin: torch.Tensor | None, rows: int, hd: int, dev: torch.device) -> None:
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    for t in (cos, sin):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (rows, hd // 2) or not t.is_contiguous() or t.device != dev):
+            raise ValueError(f"cos and sin must be contiguous float32 ({rows}, {hd // 2}) on {dev}")
+
+
+def _bf16_rows(name: str, t: torch.Tensor, rows: int | None, cols: int, dev: torch.device) -> None:
+    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != cols or t.stride(1) != 1 or t.device != dev:
+        raise ValueError(f"{name} must be bf16 rows of {cols} with unit column stride on {dev}")
+    if rows is not None and t.shape[0] != rows:
+        raise ValueError(f"{name} must have {rows} rows, not {t.shape[0]}")
+
+
+def attention_packed(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    starts: torch.Tensor,
+    max_len: int,
+    n_heads: int,
+    n_kv: int,
+    *,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal attention over prompts packed end to end: (rows, n_heads * hd).
+
+    q is (rows, n_heads * hd), k and v (rows, n_kv * hd), bf16 with any row stride (slices of the
+    fused qkv rows), head_dim 64 or 128. Sequence i is rows starts[i]:starts[i + 1] (int32, on the
+    device); its row r sees its rows 0..r only, whatever the others hold. max_len is at least the longest sequence. cos
+    and sin (rows, hd / 2) rotate q; k comes rotated (`rope_kv`). scale defaults to hd ** -0.5.
+    Rows outside every sequence are left as they are.
+    """
+    _cuda(q, k, v, starts, cos, sin, out)
+    dev = q.device
+    rows, hd = k.shape[0], k.shape[-1] // n_kv
+    _bf16_rows("q", q, rows, n_heads * hd, dev)
+    _bf16_rows("k", k, rows, n_kv * hd, dev)
+    _bf16_rows("v", v, rows, n_kv * hd, dev)
+    _ints(dev, starts=starts)
+    _tables(cos, sin, rows, hd, dev)
+    if out is None:
+        out = torch.empty(rows, n_heads * hd, dtype=torch.bfloat16, device=dev)
+    else:
+        _bf16_rows("out", out, rows, n_heads * hd, dev)
+    L.check(L.lib().so101_attention_packed(
+        q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
+        rows, starts.data_ptr(), starts.numel() - 1, max_len, n_heads, n_kv, hd, hd**-0.5 if scale is None else scale,
+        _ptr(cos), _ptr(sin), _stream(dev)), "so101_attention_packed")  # fmt: skip
+    return out
+
+
+def kv_append(
+    pages: KvPages,
+    layer: int,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    starts: torch.Tensor | None = None,
+    seqs: torch.Tensor | None = None,
+    *,
+    max_new: int = 1,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+) -> None:
+    """Quantise new keys and values into one layer of the cache.
+
+    k and v are bf16 rows (rows, n_kv * hd), any row stride. Rows starts[i]:starts[i + 1] are the last
+    tokens of sequence seqs[i], which `kv_reserve` has already counted into its length; at most
+    max_new per sequence. starts=None: one row per sequence; seqs=None: sequence i. cos and sin (rows,
+    hd / 2) rotate the keys in fp32 before they are quantised. Appending the same rows again changes nothing.
+    """
+    dev = pages.device
+    rows = k.shape[0]
+    width = pages.n_kv * pages.head_dim
+    _bf16_rows("k", k, rows, width, dev)
+    _bf16_rows("v", v, rows, width, dev)
+    _ints(dev, starts=starts, seqs=seqs)
+    _tables(cos, sin, rows, pages.head_dim, dev)
+    n = _entries(starts, seqs, rows)
+    L.check(L.lib().so101_kv_append(
+        pages.ref, layer, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), rows, _ptr(starts), _ptr(seqs), n,
+        max_new, _ptr(cos), _ptr(sin), _stream(dev)), "so101_kv_append")  # fmt: skip
+
+
+def _entries(starts: torch.Tensor | None, seqs: torch.Tensor | None, rows: int) -> int:
+    n = rows if starts is None else starts.numel() - 1
+    if n < 0 or (seqs is not None and seqs.numel() != n):
+        raise ValueError("starts has one entry more than there are sequences, seqs one per sequence")
+    return n
+
+
+def kv_read(
+    pages: KvPages,
+    layer: int,
+    starts: torch.Tensor,
+    rows: int,
+    seqs: torch.Tensor | None = None,
+    *,
+    first: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cached keys and values as bf16 rows (rows, n_kv * hd), exact: row starts[i] + r is token
+    first[i] + r (first=None: r) of sequence seqs[i] (seqs=None: i). rows is starts[-1]."""
+    dev = pages.device
+    _ints(dev, starts=starts, seqs=seqs, first=first)
+    n = _entries(starts, seqs, rows)
+    if first is not None and first.numel() != n:
+        raise ValueError("first has one entry per sequence")
+    width = pages.n_kv * pages.head_dim
+    k = torch.empty(rows, width, dtype=torch.bfloat16, device=dev)
+    v = torch.empty(rows, width, dtype=torch.bfloat16, device=dev)
+    L.check(L.lib().so101_kv_read(pages.ref, layer, starts.data_ptr(), _ptr(seqs), _ptr(first), n, rows, k.data_ptr(),
+                                  width, v.data_ptr(), width, _stream(dev)), "so101_kv_read")  # fmt: skip
+    return k, v
+
+
+def attention_pages(
+    q: torch.Tensor,
+    pages: KvPages,
+    layer: int,
+    n_heads: int,
+    starts: torch.Tensor | None = None,
+    seqs: torch.Tensor | None = None,
+    *,
+    max_q: int = 1,
+    causal: bool = True,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of each sequence's last tokens over its cached ones: (rows, n_heads * hd) bf16.
+
+    q is (rows, n_heads * hd) bf16, any row stride; rows starts[i]:starts[i + 1] are the last tokens of
+    sequence seqs[i], at most max_q of them (starts=None: one row per sequence; seqs=None: sequence i).
+    causal: token p sees tokens 0..p; otherwise every cached token (the action chunk). A row that sees
+    none is 0. cos and sin (rows, hd / 2) rotate q. scale defaults to hd ** -0.5.
+    """
+    dev = pages.device
+    rows, hd = q.shape[0], pages.head_dim
+    _bf16_rows("q", q, rows, n_heads * hd, dev)
+    _ints(dev, starts=starts, seqs=seqs)
+    _tables(cos, sin, rows, hd, dev)
+    if out is None:
+        out = torch.empty(rows, n_heads * hd, dtype=torch.bfloat16, device=dev)
+    else:
+        _bf16_rows("out", out, rows, n_heads * hd, dev)
+    n = _entries(starts, seqs, rows)
+    stream = _stream(dev)
+    ws = pages_workspace(dev, stream)
+    L.check(L.lib().so101_attention_pages(
+        q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), rows, pages.ref, layer, n_heads, _ptr(starts),
+        _ptr(seqs), n, max_q, causal, hd**-0.5 if scale is None else scale, _ptr(cos), _ptr(sin),
+        ws.partials.data_ptr(), ws.nbytes, ws.tickets.data_ptr(), ws.tickets.numel(), stream),
+        "so101_attention_pages")  # fmt: skip
+    return out
+
+
+def kv_reserve(pages: KvPages, seqs: torch.Tensor, tokens: torch.Tensor) -> None:
+    """Sequence seqs[i] grows by tokens[i] (int32, on the device): its length now, its pages from the
+    lowest free ones. The sequences are distinct. A call that cannot be met (too few free pages, a sequence past
+    `pages.max_len`) changes nothing and records ERR_PAGES (`device_status`)."""
+    _ints(pages.device, seqs=seqs, tokens=tokens)
+    if tokens.numel() != seqs.numel():
+        raise ValueError("tokens has one entry per sequence")
+    L.check(L.lib().so101_kv_reserve(pages.ref, seqs.data_ptr(), tokens.data_ptr(), seqs.numel(),
+                                     _stream(pages.device)), "so101_kv_reserve")  # fmt: skip
+
+
+def kv_free(pages: KvPages, seqs: torch.Tensor) -> None:
+    """The sequences give their pages back and are empty."""
+    _ints(pages.device, seqs=seqs)
+    L.check(L.lib().so101_kv_free(pages.ref, seqs.data_ptr(), seqs.numel(), _stream(pages.device)), "so101_kv_free")
+
+
+def kv_fork(pages: KvPages, parents: torch.Tensor, children: torch.Tensor) -> None:
+    """children[i] (distinct, empty) becomes a continuation of parents[i]: whole pages shared, a part-filled last
+    page copied in every layer. A call that cannot be met changes nothing and records ERR_PAGES."""
+    _ints(pages.device, parents=parents, children=children)
+    if parents.numel() != children.numel():
+        raise ValueError("parents and children have the same length")
+    L.check(L.lib().so101_kv_fork(pages.ref, parents.data_ptr(), children.data_ptr(), parents.numel(),
+                                  _stream(pages.device)), "so101_kv_fork")  # fmt: skip
+
+
+def kv_copy(pages: KvPages, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Pages src[i] (codes and scales, every layer) into pages dst[i]; counts and tables stay. No
+    destination may be a source or appear twice."""
+    _ints(pages.device, src=src, dst=dst)
+    if src.numel() != dst.numel():
+        raise ValueError("src and dst have the same length")
+    L.check(L.lib().so101_kv_copy(pages.ref, src.data_ptr(), dst.data_ptr(), src.numel(), _stream(pages.device)),
+            "so101_kv_copy")  # fmt: skip
+
+
+def kv_compact(pages: KvPages) -> None:
+    """The live pages move to the lowest page numbers (the k-th live page past the live count into the k-th
+    free one below it); tables and counts follow."""
+    L.check(L.lib().so101_kv_compact(pages.ref, _stream(pages.device)), "so101_kv_compact")
