@@ -9,10 +9,12 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import importlib.machinery
+import importlib.util
 import re
 from pathlib import Path
 
-from .build import LIB
+from .build import CALLS, LIB
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "so101_b200.h"
 TEXT_HEADER = HEADER.with_name("so101_b200_text.h")
@@ -170,6 +172,21 @@ def lib() -> C.CDLL:
     dll.so101_last_error.restype = C.c_char_p
     dll.so101_last_error.argtypes = []
     return dll
+
+
+@functools.cache
+def calls():
+    """The call module of the serving operators (csrc/python/calls.cpp), required like the library."""
+    lib()
+    if not CALLS.exists():
+        raise RuntimeError(f"{CALLS} is missing: build it with `python -m so101_smolvla_edge_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("_calls", str(CALLS))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_calls", loader))
+    loader.exec_module(module)
+    from . import ops
+
+    module.set_up(check, ops.pages_workspace)
+    return module
 
 
 class KernelError(RuntimeError):

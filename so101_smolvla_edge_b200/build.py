@@ -1,10 +1,11 @@
-"""Build libso101_b200.so in-tree with nvcc for sm_100a.
+"""Build libso101_b200.so in-tree with nvcc for sm_100a, and the Python call module beside it.
 
     python -m so101_smolvla_edge_b200.build [--force] [-v]
 
 Each .cu under csrc/ compiles to an object in parallel, then one shared library links them with
 the static CUDA runtime. The result lands in `so101_smolvla_edge_b200/lib/`, next to the package,
-so it travels with the source tree; nothing is installed elsewhere.
+so it travels with the source tree; nothing is installed elsewhere. `_calls.so` (csrc/python/calls.cpp:
+tensor checks and C ABI calls of the serving operators, against torch's headers) links to that library.
 """
 
 from __future__ import annotations
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -21,6 +23,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT_DIR = PKG / "lib"
 LIB = OUT_DIR / "libso101_b200.so"
+CALLS = OUT_DIR / "_calls.so"
 BUILD_DIR = PKG.parent / "_build" / "obj"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -82,7 +85,31 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode:
             raise RuntimeError(f"link failed:\n{r.stdout}{r.stderr}")
+    build_calls(force, verbose)
     return LIB
+
+
+def build_calls(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the Python call module (needs LIB) and return its path."""
+    src = CSRC / "python" / "calls.cpp"
+    if not force and not _stale(CALLS, [src, *(PKG.parent / "include").glob("*.h")]):
+        return CALLS
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    cuda = Path(nvcc()).resolve().parents[1]
+    torch_lib = Path(torch.__file__).parent / "lib"
+    inc = [*include_paths(), sysconfig.get_paths()["include"], str(cuda / "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{i}" for i in inc], str(src), "-o", str(CALLS), f"-L{OUT_DIR}", "-l:" + LIB.name, f"-L{torch_lib}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]  # fmt: skip
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode:
+        raise RuntimeError(f"g++ failed:\n{r.stdout}{r.stderr}")
+    return CALLS
 
 
 def main() -> None:

@@ -52,8 +52,10 @@ class Workspace:
     def __init__(self, device: torch.device, nbytes: int = 64 << 20, n_tickets: int = 1 << 16):
         self.partials = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
         self.tickets = torch.zeros(n_tickets, dtype=torch.int32, device=device)
-        self.nbytes, self.n_tickets = self.partials.numel() * 4, n_tickets
-        self.partials_ptr, self.tickets_ptr = self.partials.data_ptr(), self.tickets.data_ptr()
+
+    @property
+    def nbytes(self) -> int:
+        return self.partials.numel() * 4
 
 
 _WS: dict[torch.device, Workspace] = {}
@@ -473,57 +475,21 @@ def set_pdl(enable: bool) -> None:
     L.check(L.lib().so101_set_pdl(1 if enable else 0), "so101_set_pdl")
 
 
-_PAGES_WS: dict[tuple[torch.device, int], Workspace] = {}
+_PAGES_WS: dict[tuple[int, int], Workspace] = {}
 
 
-def pages_workspace(device: torch.device, stream: int) -> Workspace:
-    """The partial results of `attention_pages` on one stream (calls on several streams overlap, so
-    each has its own). It must exist before a CUDA graph is captured on the stream."""
+def pages_workspace(device: int, stream: int) -> Workspace:
+    """The partial results of `attention_pages` on one stream of a device (calls on several streams
+    overlap, so each has its own). Made by the first call on the stream: make that call before a CUDA graph
+    is captured there."""
     ws = _PAGES_WS.get((device, stream))
     if ws is None:
-        ws = _PAGES_WS[device, stream] = Workspace(device, nbytes=32 << 20)
+        ws = _PAGES_WS[device, stream] = Workspace(torch.device("cuda", device), nbytes=32 << 20)
+        L.calls().add_workspace(device, stream, ws.partials.data_ptr(), ws.nbytes, ws.tickets.data_ptr(), ws.tickets.numel())
     return ws
 
 
-# The serving operators are called once per layer and token, where a call's host time counts as much as
-# its kernel's: their checks read each tensor property once, and the stream comes without the Python
-# stream object (2.2 us to build on the measured host, against 0.07).
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
-
-
-def _int_ptr(name: str, t: torch.Tensor | None, dev: torch.device) -> int | None:
-    if t is None:
-        return None
-    if t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous() or t.device != dev:
-        raise ValueError(f"{name} must be a contiguous int32 vector on {dev}")
-    return t.data_ptr()
-
-
-def _rope_ptrs(cos: torch.Tensor | None, sin: torch.Tensor | None, rows: int, hd: int, dev: torch.device):
-    if cos is None and sin is None:
-        return None, None
-    for t in (cos, sin):
-        if t is None or t.dtype is not _F32 or t.shape != (rows, hd // 2) or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"cos and sin come together, contiguous float32 ({rows}, {hd // 2}) on {dev}")
-    return cos.data_ptr(), sin.data_ptr()
-
-
-def _bf16_rows(name: str, t: torch.Tensor, rows: int, cols: int, dev: torch.device) -> tuple[int, int]:
-    """The address and row stride of bf16 rows (rows, cols)."""
-    if t.dtype is not _BF16 or t.shape != (rows, cols) or t.device != dev:
-        raise ValueError(f"{name} must be bf16 ({rows}, {cols}) on {dev}, not {t.dtype} {tuple(t.shape)} on {t.device}")
-    ld, one = t.stride()
-    if one != 1:
-        raise ValueError(f"{name} needs unit column stride, has {t.stride()}")
-    return t.data_ptr(), ld
-
-
-def _entries(starts: torch.Tensor | None, seqs: torch.Tensor | None, rows: int) -> int:
-    n = rows if starts is None else starts.numel() - 1
-    if n < 0 or (seqs is not None and seqs.numel() != n):
-        raise ValueError("starts has one entry more than there are sequences, seqs one per sequence")
-    return n
+# The serving operators check their tensors and call the C ABI in one native step (csrc/python/calls.cpp).
 
 
 def attention_packed(
@@ -548,25 +514,7 @@ def attention_packed(
     and sin (rows, hd / 2) rotate q; k comes rotated (`rope_kv`). scale defaults to hd ** -0.5.
     Rows outside every sequence are left as they are.
     """
-    dev = q.device
-    if dev.type != "cuda":
-        raise ValueError("the B200 kernels take CUDA tensors only")
-    rows, width = k.shape
-    hd = width // n_kv
-    qp, ldq = _bf16_rows("q", q, rows, n_heads * hd, dev)
-    kp, ldk = _bf16_rows("k", k, rows, n_kv * hd, dev)
-    vp, ldv = _bf16_rows("v", v, rows, n_kv * hd, dev)
-    sp = _int_ptr("starts", starts, dev)
-    cp, np_ = _rope_ptrs(cos, sin, rows, hd, dev)
-    if out is None:
-        out = q.new_empty(rows, n_heads * hd)
-    op, ldo = _bf16_rows("out", out, rows, n_heads * hd, dev)
-    rc = L.lib().so101_attention_packed(qp, ldq, kp, ldk, vp, ldv, op, ldo, rows, sp, starts.numel() - 1, max_len,
-                                        n_heads, n_kv, hd, hd**-0.5 if scale is None else scale, cp, np_,
-                                        _raw_stream(dev.index))  # fmt: skip
-    if rc:
-        L.check(rc, "so101_attention_packed")
-    return out
+    return L.calls().attention_packed(q, k, v, starts, max_len, n_heads, n_kv, cos, sin, scale, out)
 
 
 def kv_append(
@@ -588,16 +536,7 @@ def kv_append(
     max_new per sequence. starts=None: one row per sequence; seqs=None: sequence i. cos and sin (rows,
     hd / 2) rotate the keys in fp32 before they are quantised. Appending the same rows again changes nothing.
     """
-    dev, hd = pages.device, pages.head_dim
-    rows, width = k.shape[0], pages.n_kv * hd
-    kp, ldk = _bf16_rows("k", k, rows, width, dev)
-    vp, ldv = _bf16_rows("v", v, rows, width, dev)
-    cp, np_ = _rope_ptrs(cos, sin, rows, hd, dev)
-    n = _entries(starts, seqs, rows)
-    rc = L.lib().so101_kv_append(pages.ref, layer, kp, ldk, vp, ldv, rows, _int_ptr("starts", starts, dev),
-                                 _int_ptr("seqs", seqs, dev), n, max_new, cp, np_, _raw_stream(dev.index))  # fmt: skip
-    if rc:
-        L.check(rc, "so101_kv_append")
+    L.calls().kv_append(pages.handle, layer, k, v, starts, seqs, max_new, cos, sin)
 
 
 def kv_read(
@@ -611,19 +550,7 @@ def kv_read(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Cached keys and values as bf16 rows (rows, n_kv * hd), exact: row starts[i] + r is token
     first[i] + r (first=None: r) of sequence seqs[i] (seqs=None: i). rows is starts[-1]."""
-    dev = pages.device
-    n = _entries(starts, seqs, rows)
-    if first is not None and first.numel() != n:
-        raise ValueError("first has one entry per sequence")
-    width = pages.n_kv * pages.head_dim
-    both = torch.empty((2, rows, width), dtype=_BF16, device=dev)
-    at = both.data_ptr()
-    rc = L.lib().so101_kv_read(pages.ref, layer, _int_ptr("starts", starts, dev), _int_ptr("seqs", seqs, dev),
-                               _int_ptr("first", first, dev), n, rows, at, width, at + 2 * rows * width, width,
-                               _raw_stream(dev.index))  # fmt: skip
-    if rc:
-        L.check(rc, "so101_kv_read")
-    return both[0], both[1]
+    return L.calls().kv_read(pages.handle, layer, starts, rows, seqs, first)
 
 
 def attention_pages(
@@ -648,64 +575,34 @@ def attention_pages(
     causal: token p sees tokens 0..p; otherwise every cached token (the action chunk). A row that sees
     none is 0. cos and sin (rows, hd / 2) rotate q. scale defaults to hd ** -0.5.
     """
-    dev, hd = pages.device, pages.head_dim
-    rows, width = q.shape[0], n_heads * hd
-    qp, ldq = _bf16_rows("q", q, rows, width, dev)
-    cp, np_ = _rope_ptrs(cos, sin, rows, hd, dev)
-    if out is None:
-        out = q.new_empty(rows, width)
-    op, ldo = _bf16_rows("out", out, rows, width, dev)
-    n = _entries(starts, seqs, rows)
-    stream = _raw_stream(dev.index)
-    ws = pages_workspace(dev, stream)
-    rc = L.lib().so101_attention_pages(qp, ldq, op, ldo, rows, pages.ref, layer, n_heads, _int_ptr("starts", starts, dev),
-                                       _int_ptr("seqs", seqs, dev), n, max_q, causal,
-                                       hd**-0.5 if scale is None else scale, cp, np_, ws.partials_ptr, ws.nbytes,
-                                       ws.tickets_ptr, ws.n_tickets, stream)  # fmt: skip
-    if rc:
-        L.check(rc, "so101_attention_pages")
-    return out
+    return L.calls().attention_pages(q, pages.handle, layer, n_heads, starts, seqs, max_q, causal, cos, sin, scale, out)
 
 
 def kv_reserve(pages: KvPages, seqs: torch.Tensor, tokens: torch.Tensor) -> None:
     """Sequence seqs[i] grows by tokens[i] (int32, on the device): its length now, its pages from the
     lowest free ones. The sequences are distinct. A call that cannot be met (too few free pages, a sequence past
     `pages.max_len`) changes nothing and records ERR_PAGES (`device_status`)."""
-    dev = pages.device
-    if tokens.numel() != seqs.numel():
-        raise ValueError("tokens has one entry per sequence")
-    L.check(L.lib().so101_kv_reserve(pages.ref, _int_ptr("seqs", seqs, dev), _int_ptr("tokens", tokens, dev),
-                                     seqs.numel(), _raw_stream(dev.index)), "so101_kv_reserve")  # fmt: skip
+    L.calls().kv_reserve(pages.handle, seqs, tokens)
 
 
 def kv_free(pages: KvPages, seqs: torch.Tensor) -> None:
     """The sequences give their pages back and are empty."""
-    dev = pages.device
-    L.check(L.lib().so101_kv_free(pages.ref, _int_ptr("seqs", seqs, dev), seqs.numel(), _raw_stream(dev.index)),
-            "so101_kv_free")  # fmt: skip
+    L.calls().kv_free(pages.handle, seqs)
 
 
 def kv_fork(pages: KvPages, parents: torch.Tensor, children: torch.Tensor) -> None:
     """children[i] (distinct, empty) becomes a continuation of parents[i]: whole pages shared, a part-filled last
     page copied in every layer. A call that cannot be met changes nothing and records ERR_PAGES."""
-    dev = pages.device
-    if parents.numel() != children.numel():
-        raise ValueError("parents and children have the same length")
-    L.check(L.lib().so101_kv_fork(pages.ref, _int_ptr("parents", parents, dev), _int_ptr("children", children, dev),
-                                  parents.numel(), _raw_stream(dev.index)), "so101_kv_fork")  # fmt: skip
+    L.calls().kv_fork(pages.handle, parents, children)
 
 
 def kv_copy(pages: KvPages, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Pages src[i] (codes and scales, every layer) into pages dst[i]; counts and tables stay. No
     destination may be a source or appear twice."""
-    dev = pages.device
-    if src.numel() != dst.numel():
-        raise ValueError("src and dst have the same length")
-    L.check(L.lib().so101_kv_copy(pages.ref, _int_ptr("src", src, dev), _int_ptr("dst", dst, dev), src.numel(),
-                                  _raw_stream(dev.index)), "so101_kv_copy")  # fmt: skip
+    L.calls().kv_copy(pages.handle, src, dst)
 
 
 def kv_compact(pages: KvPages) -> None:
     """The live pages move to the lowest page numbers (the k-th live page past the live count into the k-th
     free one below it); tables and counts follow."""
-    L.check(L.lib().so101_kv_compact(pages.ref, _raw_stream(pages.device.index)), "so101_kv_compact")
+    L.calls().kv_compact(pages.handle)

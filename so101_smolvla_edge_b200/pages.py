@@ -72,7 +72,8 @@ class KvPages:
         L.check(L.lib().so101_kv_scratch(C.byref(self.desc), C.byref(ints)), "so101_kv_scratch")
         self.scratch = torch.zeros(ints.value, dtype=torch.int32, device=k.device)
         self.desc.scratch = self.scratch.data_ptr()
-        self.ref = C.byref(self.desc)
+        # what the calls take: the descriptor's address and the device
+        self.handle = (C.addressof(self.desc), k.device.index)
 
     @property
     def max_len(self) -> int:
