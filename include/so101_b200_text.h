@@ -38,8 +38,8 @@ SO101_API int so101_attention_packed(const void* q, int64_t ldq, const void* k, 
  * scales: k_scale / v_scale [layer][page][kv head] fp32, one power of two per page and head, the
  * value being code * scale. refs[p] counts the sequences that hold page p (0: free). table rows
  * hold -1 past a sequence's pages. page 16, 32 or 64; hd 64 or 128; k, v, k_scale, v_scale
- * 16-byte aligned. scratch: so101_kv_scratch ints, used by reserve, fork and compact, which must
- * be ordered on one stream. */
+ * 16-byte aligned. scratch: so101_kv_scratch ints, zero before the first call, used by
+ * reserve, fork and compact, which must be ordered on one stream. */
 typedef struct so101_kv_pages {
   int8_t* k;
   int8_t* v;

@@ -126,9 +126,10 @@ __device__ __forceinline__ void add_scaled(float4& y, float w, const float4& x) 
 
 // Where the CTAs' work lies. A problem is (list entry, tile of ROWS query rows, kv head); its keys make
 // steps of kStep, at least one, counted by the sequence's length. All problems' steps, end to end, are dealt
-// out in equal runs, one per CTA: whatever the lengths, every CTA reads about as many keys. A cut
-// that falls within an eighth of a run of a problem's end moves there (a part of a problem costs its rows
-// written and read again; an eighth of a run costs less).
+// out in equal runs, one per CTA: whatever the lengths, every CTA reads about as many keys. A cut within an
+// eighth of a run, or two steps, of a problem's end moves there: a part costs its rows written and read again and
+// the wait for the last of them, about as long as two steps (64 sequences of 1000 keys, runs of three
+// steps: 16.0 us, 20.1 with every cut where it falls; longer sequences take the same time either way).
 struct PagesPlan {
   int entry, first;  // the entry that holds the CTA's first step, and the step at which it begins
   int run, slack, total;
@@ -172,7 +173,7 @@ __device__ __forceinline__ PagesPlan pages_plan(const PagesArgs& a, int* shared)
   PagesPlan p;
   p.total = shared[0] + shared[1] + shared[2] + shared[3];
   p.run = max(1, (p.total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-  p.slack = p.run / 8;
+  p.slack = max(p.run / 8, min(2, p.run - 1));
   p.entry = p.first = p.begin = p.end = 0;
   const int cut0 = static_cast<int>(blockIdx.x) * p.run, cut1 = cut0 + p.run;
   __syncthreads();
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
   int entry = plan.entry, entry_first = plan.first;
   int at = plan.begin;  // the next step of this CTA's run
   int used = 0;         // tiles that this ring has taken (stages and phases)
+  int issued = 0;       // and asked for
   bool ok = true;
   while (at < plan.end && entry < a.n_seqs) {
     // ---- the problem that step `at` belongs to, and the part of it in this CTA's run
@@ -316,6 +318,7 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
         record_error(a.status, SO101_ERR_PAGES);
         mine = false;
       }
+      issued = used + i + 1;
       const int runs = __popc(__ballot_sync(0xffffffffu, mine));
       const uint32_t bytes = static_cast<uint32_t>(GRAN * HD);
       if (lane == 0) mbar_arrive_expect_tx(&my_bars[st], 2u * bytes * runs);
@@ -580,6 +583,9 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
       if (more) put_scales(i + kStages - 1);
       ring_sync();  // the stage is read: the next load may fill it
     }
+    if (!ok && roww == 0)  // copies in flight land before the ring's memory is used otherwise
+      for (int n = max(0, issued - kStages); n < issued; ++n)
+        mbar_wait(&my_bars[n % kStages], static_cast<uint32_t>(n / kStages) & 1u, a.status);
     used += tiles;
     __syncthreads();  // every ring's tiles have landed and been read
 

@@ -1,22 +1,29 @@
 // The pages of the 8-bit cache: taken (so101_kv_reserve), given back (so101_kv_free), shared and copied
 // (so101_kv_fork, so101_kv_copy) and moved together (so101_kv_compact).
 //
-// All on the device, so that a serving loop neither waits for the GPU nor mirrors its tables. A plan
-// kernel of one CTA orders what has to be ordered (free pages by number, list entries by place) with
-// prefix sums: the same inputs give the same pages, and a call that cannot be met changes nothing.
-// It leaves a list of page moves in the scratch ints, which a second launch over the whole GPU
-// carries out: a page is n_layers x 2 runs of n_kv * page * hd bytes (20 KB for five heads of 64 and
-// 64 slots), read and written once in 16-byte pieces, which the HBM copy rate bounds.
+// All on the device, so that a serving loop neither waits for the GPU nor mirrors its tables. One CTA
+// orders what has to be ordered (free pages by number, list entries by place) with prefix sums: the
+// same inputs give the same pages, and a call that cannot be met changes nothing. Fork and compact leave
+// a list of page moves in the scratch ints, which all CTAs of the same launch then carry out: the CTA that
+// arrives first plans, the others wait (bounded) for its flag. A page is n_layers x 2 runs of
+// n_kv * page * hd bytes (20 KB for five heads of 64 and 64 slots); the runs go through shared
+// memory in bulk copies, eight in flight per SM, bounded by the HBM copy rate.
+#include <atomic>
+
 #include "kv_pages.cuh"
 
 namespace so101 {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 512;
 
-// Scratch ints: [0] number of moves, then src[most], dst[most] (most = max(n_pages, max_seqs)), then
+// Scratch ints: number of moves, arrivals, the plan's flag and departures (the last three zero between
+// calls), then src[most], dst[most] (most = max(n_pages, max_seqs)), then
 // remap[n_pages] and the parents' lengths / running offsets [max_seqs].
 struct Scratch {
   int* moves;
+  int* arrived;
+  int* ready;
+  int* left;
   int* src;
   int* dst;
   int* remap;
@@ -29,6 +36,9 @@ __device__ __forceinline__ Scratch scratch_of(const KvPages& c) {
   const long long most = scratch_most(c);
   Scratch s;
   s.moves = c.scratch;
+  s.arrived = c.scratch + 1;
+  s.ready = c.scratch + 2;
+  s.left = c.scratch + 3;
   s.src = c.scratch + 4;
   s.dst = s.src + most;
   s.remap = s.dst + most;
@@ -48,7 +58,7 @@ __device__ __forceinline__ int block_scan(int x, int& total, int* warp_sums) {
   if (lane == 31) warp_sums[warp] = inc;
   __syncthreads();
   if (warp == 0) {
-    int w = warp_sums[lane];
+    int w = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, w, d);
@@ -58,7 +68,7 @@ __device__ __forceinline__ int block_scan(int x, int& total, int* warp_sums) {
   }
   __syncthreads();
   const int before = warp ? warp_sums[warp - 1] : 0;
-  total = warp_sums[31];
+  total = warp_sums[kPlanThreads / 32 - 1];
   __syncthreads();
   return before + inc - x;
 }
@@ -166,11 +176,8 @@ __global__ void __launch_bounds__(kFreeThreads) kv_free_kernel(const ListArgs g)
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ListArgs g) {
-  __shared__ int warp_sums[32];
+__device__ __forceinline__ void plan_fork(const ListArgs& g, int* warp_sums) {
   __shared__ int bad;
-  grid_dep_launch();
-  grid_dep_wait();
   const KvPages& c = g.c;
   const Scratch s = scratch_of(c);
   if (threadIdx.x == 0) {
@@ -233,10 +240,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ListArgs
 }
 
 // Live pages past the live count into the free ones below it, both ascending.
-__global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const ListArgs g) {
-  __shared__ int warp_sums[32];
-  grid_dep_launch();
-  grid_dep_wait();
+__device__ __forceinline__ void plan_compact(const ListArgs& g, int* warp_sums) {
   const KvPages& c = g.c;
   const Scratch s = scratch_of(c);
   int live = 0;
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const ListA
     const bool in = p < c.n_pages;
     const bool used = in && c.refs[p] > 0;
     const int move = used && p >= total, hole = in && !used && p < total;
-    int sum;  // both counts in one scan: at most 1024 of each per turn
+    int sum;  // both counts in one scan: at most 512 of each per turn
     const int off = block_scan(move | hole << 16, sum, warp_sums);
     if (move) s.src[high + (off & 0xFFFF)] = p;
     if (hole) s.dst[holes + (off >> 16)] = p;
@@ -267,72 +271,172 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const ListA
   if (threadIdx.x == 0) *s.moves = high;
 }
 
-constexpr int kMoveThreads = 256;
-constexpr int kMovePieces = 4;  // 16-byte pieces that a thread holds at once
+enum { kMoveCopy, kMoveFork, kMoveCompact };
+constexpr int kMoveStages = 8;
+constexpr int kMoveChunk = 16384;  // bytes of a run that go at once, at most
 
-// The moves of the list, one unit at a time per CTA: unit u is (move, layer, keys or values, part);
-// with `remap`, the table entries too. src / dst given: n pairs; null: the scratch list.
-__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const ListArgs g, const int remap) {
-  grid_dep_launch();
-  grid_dep_wait();
+constexpr int kMoveBatch = 512;  // units whose addresses the CTA works out together
+
+struct MoveSmem {
+  uint8_t data[kMoveStages][kMoveChunk];
+  const int8_t* from[kMoveBatch];
+  int8_t* to[kMoveBatch];
+  int bytes[kMoveBatch];  // 0: a page out of range
+  uint64_t full[kMoveStages];
+};
+
+__device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void bulk_out(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;" ::"l"(dst),
+               "r"(src), "r"(bytes)
+               : "memory");
+}
+
+__device__ __forceinline__ int ld_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_release(int* p, int v) {
+  asm volatile("st.release.gpu.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
+// Plan (fork, compact), then move. Unit u of the moves is (move, layer, keys or values, chunk); CTA b
+// takes units b, b + gridDim.x, ...: all its threads work out the addresses of a batch of them (a single
+// thread that looks each page number up itself moves a unit in 2 us: 266 us for 335 MB), then
+// thread 0 keeps kMoveStages / 2 loads ahead of the stores.
+template <int MODE>
+__global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs g) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  MoveSmem& sm = *reinterpret_cast<MoveSmem*>(smem_raw);
+  __shared__ int warp_sums[32];
+  __shared__ int shared;
   const KvPages& c = g.c;
   const Scratch s = scratch_of(c);
-  const int* src = g.a ? g.a : s.src;
-  const int* dst = g.a ? g.b : s.dst;
-  const int moves = g.a ? g.n : *s.moves;
-  const int pieces = c.n_kv * c.page * c.hd / 16;  // of a page, per layer, keys or values
-  constexpr int kUnit = kMoveThreads * kMovePieces;
-  const int parts = (pieces + kUnit - 1) / kUnit;
-  const long long units = static_cast<long long>(moves) * c.n_layers * 2 * parts;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int part = static_cast<int>(u % parts);
-    const long long w = u / parts;
-    const int which = static_cast<int>(w & 1);
-    const int layer = static_cast<int>((w >> 1) % c.n_layers);
-    const int k = static_cast<int>((w >> 1) / c.n_layers);
-    const int from = src[k], to = dst[k];
-    if (from < 0 || from >= c.n_pages || to < 0 || to >= c.n_pages) {
-      if (threadIdx.x == 0) record_error(g.status, SO101_ERR_PAGES);
-      continue;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kMoveStages; ++i) mbar_init(&sm.full[i], 1);
+    fence_mbar_init();
+  }
+  grid_dep_launch();
+  grid_dep_wait();
+  if (MODE != kMoveCopy) {
+    // the first CTA to arrive plans: it is running, so the others may wait for it
+    if (threadIdx.x == 0) shared = atomicAdd(s.arrived, 1);
+    __syncthreads();
+    if (shared == 0) {
+      if (MODE == kMoveFork) plan_fork(g, warp_sums);
+      else plan_compact(g, warp_sums);
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        __threadfence();
+        st_release(s.ready, 1);
+      }
+    } else if (threadIdx.x == 0) {
+      const uint64_t t0 = globaltimer();
+      while (!ld_acquire(s.ready)) {
+        if (globaltimer() - t0 > kWaitLimitNs) {
+          record_error(g.status, SO101_ERR_TIMEOUT);
+          break;
+        }
+        __nanosleep(100);
+      }
     }
-    int8_t* codes = which ? c.v : c.k;
-    const uint4* x = reinterpret_cast<const uint4*>(codes + kv_code_at(c, layer, from, 0));
-    uint4* y = reinterpret_cast<uint4*>(codes + kv_code_at(c, layer, to, 0));
-    uint4 t[kMovePieces];
-#pragma unroll
-    for (int i = 0; i < kMovePieces; ++i) {
-      const int p = part * kUnit + i * kMoveThreads + static_cast<int>(threadIdx.x);
-      if (p < pieces) t[i] = x[p];
-    }
-#pragma unroll
-    for (int i = 0; i < kMovePieces; ++i) {
-      const int p = part * kUnit + i * kMoveThreads + static_cast<int>(threadIdx.x);
-      if (p < pieces) y[p] = t[i];
-    }
-    if (part == 0) {
+    __syncthreads();
+  }
+  const bool planned = MODE == kMoveCopy || ld_acquire(s.ready);
+  const int* src = MODE == kMoveCopy ? g.a : s.src;
+  const int* dst = MODE == kMoveCopy ? g.b : s.dst;
+  const int moves = MODE == kMoveCopy ? g.n : planned ? __ldcg(s.moves) : 0;
+  const int run = c.n_kv * c.page * c.hd;  // bytes per move, layer, keys or values
+  const int chunks = (run + kMoveChunk - 1) / kMoveChunk;
+  const int chunk = ((run + chunks - 1) / chunks + 15) / 16 * 16;
+  const long long units = static_cast<long long>(moves) * c.n_layers * 2 * chunks;
+  // the scales, and after a compaction the tables: by the warps that do not copy
+  auto small_work = [&]() {
+    const int t = static_cast<int>(threadIdx.x) - 32, step = kPlanThreads - 32;
+    const long long scales = static_cast<long long>(moves) * c.n_layers * c.n_kv * 2;
+    for (long long e = static_cast<long long>(blockIdx.x) * step + t; e < scales;
+         e += static_cast<long long>(gridDim.x) * step) {
+      const int which = static_cast<int>(e & 1);
+      const int h = static_cast<int>((e >> 1) % c.n_kv);
+      const long long w = (e >> 1) / c.n_kv;
+      const int layer = static_cast<int>(w % c.n_layers), k = static_cast<int>(w / c.n_layers);
+      const int from = __ldcg(src + k), to = __ldcg(dst + k);
+      if (from < 0 || from >= c.n_pages || to < 0 || to >= c.n_pages) continue;
       float* sc = which ? c.v_scale : c.k_scale;
-      for (int h = threadIdx.x; h < c.n_kv; h += kMoveThreads)
-        sc[kv_scale_at(c, layer, to, h)] = sc[kv_scale_at(c, layer, from, h)];
+      sc[kv_scale_at(c, layer, to, h)] = sc[kv_scale_at(c, layer, from, h)];
+    }
+    if (MODE == kMoveCompact && planned) {
+      const long long entries = static_cast<long long>(c.max_seqs) * c.max_pages;
+      for (long long e = static_cast<long long>(blockIdx.x) * step + t; e < entries;
+           e += static_cast<long long>(gridDim.x) * step) {
+        const int id = c.table[e];
+        if (id >= 0 && id < c.n_pages) c.table[e] = __ldcg(s.remap + id);
+      }
+    }
+  };
+  const long long mine = units > blockIdx.x ? (units - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+  constexpr int kAhead = kMoveStages / 2;
+  bool ok = true;
+  for (long long i0 = 0; i0 < mine || i0 == 0; i0 += kMoveBatch) {
+    const int n = static_cast<int>(max(0LL, min(static_cast<long long>(kMoveBatch), mine - i0)));
+    __syncthreads();  // thread 0 is done with the batch before
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+      const long long u = blockIdx.x + (i0 + i) * gridDim.x, w = u / chunks;
+      const int off = static_cast<int>(u % chunks) * chunk;
+      const int layer = static_cast<int>((w >> 1) % c.n_layers), k = static_cast<int>((w >> 1) / c.n_layers);
+      const int from = __ldcg(src + k), to = __ldcg(dst + k);
+      const bool valid = from >= 0 && from < c.n_pages && to >= 0 && to < c.n_pages;
+      if (!valid) record_error(g.status, SO101_ERR_PAGES);
+      int8_t* codes = (w & 1) ? c.v : c.k;
+      sm.from[i] = codes + (valid ? kv_code_at(c, layer, from, 0) + off : 0);
+      sm.to[i] = codes + (valid ? kv_code_at(c, layer, to, 0) + off : 0);
+      sm.bytes[i] = valid ? min(chunk, run - off) : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      // stage and phase of unit i of the batch: its batch's predecessors are whole batches, so i serves
+      static_assert(kMoveBatch % (2 * kMoveStages) == 0, "a batch ends on an even phase");
+      for (int i = 0; i < n + kAhead && ok; ++i) {
+        if (i < n) {  // load unit i; its stage's last store has read it
+          asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kMoveStages - kAhead - 1) : "memory");
+          const int st = i % kMoveStages;
+          const uint32_t bytes = static_cast<uint32_t>(sm.bytes[i]);
+          mbar_arrive_expect_tx(&sm.full[st], bytes);
+          if (bytes) bulk_in(smem_u32(sm.data[st]), sm.from[i], bytes, &sm.full[st]);
+        }
+        const int j = i - kAhead;
+        if (j >= 0) {  // store unit j
+          ok = mbar_wait(&sm.full[j % kMoveStages], static_cast<uint32_t>(j / kMoveStages) & 1u, g.status);
+          if (ok && sm.bytes[j])
+            bulk_out(sm.to[j], smem_u32(sm.data[j % kMoveStages]), static_cast<uint32_t>(sm.bytes[j]));
+          else
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // the groups count units
+          if (!ok)  // a wait ran out: the loads still in flight must land before this CTA's shared memory goes
+            for (int k = j + 1; k <= i && k < n; ++k)
+              mbar_wait(&sm.full[k % kMoveStages], static_cast<uint32_t>(k / kMoveStages) & 1u, g.status);
+        }
+      }
+    } else if (threadIdx.x >= 32 && i0 == 0) {
+      small_work();
     }
   }
-  if (remap) {
-    const long long entries = static_cast<long long>(c.max_seqs) * c.max_pages;
-    for (long long e = static_cast<long long>(blockIdx.x) * kMoveThreads + threadIdx.x; e < entries;
-         e += static_cast<long long>(gridDim.x) * kMoveThreads) {
-      const int id = c.table[e];
-      if (id >= 0 && id < c.n_pages) c.table[e] = s.remap[id];
+  if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (MODE != kMoveCopy) {
+    __syncthreads();
+    if (threadIdx.x == 0 && atomicAdd(s.left, 1) == static_cast<int>(gridDim.x) - 1) {
+      *s.arrived = 0;
+      *s.left = 0;
+      *s.ready = 0;
     }
   }
 }
 
 namespace {
-
-int sm_count() {
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
-  return n;
-}
 
 ListArgs list_args(const KvPages* c, const int* a, const int* b, int n) {
   ListArgs g;
@@ -344,14 +448,25 @@ ListArgs list_args(const KvPages* c, const int* a, const int* b, int n) {
   return g;
 }
 
-// The copies of at most `most` moves (an upper bound is enough: the list's own length rules).
-int move_pages(const ListArgs& g, long long most, int remap, cudaStream_t stream) {
-  const long long pieces = static_cast<long long>(g.c.n_kv) * g.c.page * g.c.hd / 16;
-  const long long parts = (pieces + kMoveThreads * kMovePieces - 1) / (kMoveThreads * kMovePieces);
-  const long long units = most * g.c.n_layers * 2 * parts;
-  const long long full = static_cast<long long>(sm_count()) * 8;
+// At most `most` moves (an upper bound is enough: the list's own length rules), one CTA per SM.
+template <int MODE>
+int move_pages(const ListArgs& g, long long most, cudaStream_t stream) {
+  static std::atomic<int> sms[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return SO101_ERR_DRIVER;
+  int full = sms[dev].load();
+  if (!full) {
+    cudaError_t e = cudaFuncSetAttribute(kv_move_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(sizeof(MoveSmem)));
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&full, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return launch_error(e);
+    sms[dev].store(full);
+  }
+  const long long run = static_cast<long long>(g.c.n_kv) * g.c.page * g.c.hd;
+  const long long units = most * g.c.n_layers * 2 * ((run + kMoveChunk - 1) / kMoveChunk);
   const dim3 grid(static_cast<unsigned>(units < full ? units : full));
-  return launch_kernel(kv_move_kernel, grid, dim3(kMoveThreads), 0, stream, g, remap);
+  return launch_kernel(kv_move_kernel<MODE>, grid, dim3(kPlanThreads), sizeof(MoveSmem), stream, g);
 }
 
 }  // namespace
@@ -385,20 +500,16 @@ extern "C" int so101_kv_fork(const so101_kv_pages* c, const int* parents, const 
                              cudaStream_t stream) {
   if (!kv_pages_ok(c) || n < 0 || n > c->max_seqs || (n > 0 && (!parents || !children))) return SO101_ERR_ARG;
   if (n == 0) return SO101_OK;
-  const int rc = launch_kernel(kv_fork_kernel, dim3(1), dim3(kPlanThreads), 0, stream,
-                               list_args(c, parents, children, n));
-  return rc ? rc : move_pages(list_args(c, nullptr, nullptr, 0), n, 0, stream);
+  return move_pages<kMoveFork>(list_args(c, parents, children, n), n, stream);
 }
 
 extern "C" int so101_kv_copy(const so101_kv_pages* c, const int* src, const int* dst, int n, cudaStream_t stream) {
   if (!kv_pages_ok(c) || n < 0 || n > c->n_pages || (n > 0 && (!src || !dst))) return SO101_ERR_ARG;
   if (n == 0) return SO101_OK;
-  return move_pages(list_args(c, src, dst, n), n, 0, stream);
+  return move_pages<kMoveCopy>(list_args(c, src, dst, n), n, stream);
 }
 
 extern "C" int so101_kv_compact(const so101_kv_pages* c, cudaStream_t stream) {
   if (!kv_pages_ok(c)) return SO101_ERR_ARG;
-  const ListArgs g = list_args(c, nullptr, nullptr, 0);
-  const int rc = launch_kernel(kv_compact_kernel, dim3(1), dim3(kPlanThreads), 0, stream, g);
-  return rc ? rc : move_pages(g, c->n_pages, 1, stream);
+  return move_pages<kMoveCompact>(list_args(c, nullptr, nullptr, 0), c->n_pages, stream);
 }
