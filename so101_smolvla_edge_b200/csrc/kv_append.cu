@@ -84,35 +84,50 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendA
   }
   if (blockIdx.x == gridDim.x - 1 && len > (at + 1) * c.page && threadIdx.x == 0)
     record_error(a.status, SO101_ERR_PAGES);
-  const int id = c.table[static_cast<long long>(seq) * c.max_pages + at];
-  if (id < 0 || id >= c.n_pages) {
-    if (threadIdx.x == 0) record_error(a.status, SO101_ERR_PAGES);
-    return;
-  }
   const int held = lo - at * c.page;  // older tokens of the page
   const __nv_bfloat16* src = a.x[which] + static_cast<long long>(row0 + lo - old) * a.ld[which] + head * HD;
   const long long ld = a.ld[which];
   const bool turn = which == 0 && a.cos != nullptr;
   const int pairs = (hi - lo) * kPairs;
+  // the page's number is looked up while the rows are on their way
+  uint4 u[kMost][2];
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const int p = threadIdx.x + i * kAppendThreads;
+    if (p < pairs) {
+      const __nv_bfloat16* row = src + p / kPairs * ld + p % kPairs * 8;
+      u[i][0] = __ldg(reinterpret_cast<const uint4*>(row));
+      u[i][1] = __ldg(reinterpret_cast<const uint4*>(row + HD / 2));
+    }
+  }
+  const int id = c.table[static_cast<long long>(seq) * c.max_pages + at];
+  if (id < 0 || id >= c.n_pages) {
+    if (threadIdx.x == 0) record_error(a.status, SO101_ERR_PAGES);
+    return;
+  }
+  float* scale = (which ? c.v_scale : c.k_scale) + kv_scale_at(c, a.layer, id, head);
+  const float was = held ? *scale : 0.f;
   float x[kMost][2][8];
   uint32_t big = 0u;
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
     const int p = threadIdx.x + i * kAppendThreads;
     if (p < pairs) {
-      const int r = p / kPairs, d = p % kPairs * 8;
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(src + r * ld + d));
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + r * ld + d + HD / 2));
-      unpack8(u, x[i][0]);
-      unpack8(w, x[i][1]);
+      unpack8(u[i][0], x[i][0]);
+      unpack8(u[i][1], x[i][1]);
       if (turn) {
-        const long long t = static_cast<long long>(row0 + lo - old + r) * (HD / 2) + d;
+        const long long t = static_cast<long long>(row0 + lo - old + p / kPairs) * (HD / 2) + p % kPairs * 8;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float cs = __ldg(a.cos + t + e), sn = __ldg(a.sin + t + e);
-          const float u0 = x[i][0][e], u1 = x[i][1][e];
-          x[i][0][e] = __fsub_rn(__fmul_rn(u0, cs), __fmul_rn(u1, sn));
-          x[i][1][e] = __fadd_rn(__fmul_rn(u1, cs), __fmul_rn(u0, sn));
+        for (int e0 = 0; e0 < 8; e0 += 4) {
+          const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + t + e0));
+          const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin + t + e0));
+          const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float u0 = x[i][0][e0 + e], u1 = x[i][1][e0 + e];
+            x[i][0][e0 + e] = __fsub_rn(__fmul_rn(u0, cv[e]), __fmul_rn(u1, sv[e]));
+            x[i][1][e0 + e] = __fadd_rn(__fmul_rn(u1, cv[e]), __fmul_rn(u0, sv[e]));
+          }
         }
       }
       // magnitudes compare as integers; a NaN is past infinity
@@ -123,8 +138,6 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendA
   }
   big = __reduce_max_sync(0xffffffffu, big);
   if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = big;
-  float* scale = (which ? c.v_scale : c.k_scale) + kv_scale_at(c, a.layer, id, head);
-  const float was = held ? *scale : 0.f;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kAppendThreads / 32; ++w) big = max(big, warp_max[w]);
@@ -169,42 +182,58 @@ struct ReadArgs {
   int* status;
 };
 
-constexpr int kReadRows = 16, kReadThreads = 128;
+constexpr int kReadRows = 8, kReadThreads = 256;
 
-// 16 rows per CTA; a thread takes 16 codes of a row (one 16-byte load, two 16-byte stores).
+// 8 rows per CTA. Where the rows lie is worked out once, a thread per row (the sequence by counting the
+// starts at or before it, in one barrier per 256 of them); then a thread takes 16 codes of a row at a
+// time: one 16-byte load, two 16-byte stores. Latency bounds a small call (64 rows: 3.6 us; looking the
+// sequence, length and page up again for each piece took 11 us), the stores' bandwidth a large one.
 template <int HD>
 __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const ReadArgs a) {
-  __shared__ int found;
+  __shared__ int page_of[kReadRows], slot_of[kReadRows];
   grid_dep_launch();
   grid_dep_wait();
   const KvPages& c = a.c;
   const int r0 = blockIdx.x * kReadRows;
-  const int s0 = find_sequence(a.starts, a.n_seqs, r0, &found);
-  constexpr int kPieces = HD / 16;
-  const int per_row = 2 * c.n_kv * kPieces;
-  for (int p = threadIdx.x; p < kReadRows * per_row; p += kReadThreads) {
-    const int row = r0 + p / per_row;
-    int q = p % per_row;
-    const int d = q % kPieces * 16;
-    q /= kPieces;
-    const int head = q % c.n_kv, which = q / c.n_kv;
-    if (row >= a.rows) continue;
+  int s0 = -1;
+  for (int i0 = 0; i0 <= a.n_seqs; i0 += kReadThreads) {
+    const int i = i0 + static_cast<int>(threadIdx.x);
+    s0 += __syncthreads_count(i <= a.n_seqs && __ldg(a.starts + i) <= r0);
+  }
+  if (threadIdx.x < kReadRows) {
+    const int row = r0 + static_cast<int>(threadIdx.x);
+    int id = -1, slot = 0;
     int i = s0;
     while (i < a.n_seqs && (i < 0 || __ldg(a.starts + i + 1) <= row)) ++i;
-    if (i < 0 || i >= a.n_seqs) continue;  // a row outside every sequence
-    const int seq = a.seqs ? __ldg(a.seqs + i) : i;
-    const int tok = (a.first ? __ldg(a.first + i) : 0) + row - __ldg(a.starts + i);
-    if (seq < 0 || seq >= c.max_seqs || tok < 0 || tok >= c.lengths[seq] || tok >= c.max_pages * c.page) {
-      record_error(a.status, SO101_ERR_PAGES);
-      continue;
+    if (row < a.rows && i >= 0 && i < a.n_seqs) {  // else a row outside every sequence
+      const int seq = a.seqs ? __ldg(a.seqs + i) : i;
+      const int tok = (a.first ? __ldg(a.first + i) : 0) + row - __ldg(a.starts + i);
+      const bool there = seq >= 0 && seq < c.max_seqs && tok >= 0 && tok < c.max_pages * c.page;
+      if (there) {
+        const int len = c.lengths[seq];
+        id = c.table[static_cast<long long>(seq) * c.max_pages + tok / c.page];
+        slot = tok % c.page;
+        if (tok >= len || id >= c.n_pages) id = -1;
+      }
+      if (id < 0) record_error(a.status, SO101_ERR_PAGES);
     }
-    const int id = c.table[static_cast<long long>(seq) * c.max_pages + tok / c.page];
-    if (id < 0 || id >= c.n_pages) {
-      record_error(a.status, SO101_ERR_PAGES);
-      continue;
-    }
+    page_of[threadIdx.x] = id;
+    slot_of[threadIdx.x] = slot;
+  }
+  __syncthreads();
+  constexpr int kPieces = HD / 16;
+  const int per_row = 2 * c.n_kv * kPieces;
+#pragma unroll 2
+  for (int p = threadIdx.x; p < kReadRows * per_row; p += kReadThreads) {
+    const int r = p / per_row;
+    int q = p - r * per_row;
+    const int d = q % kPieces * 16;
+    q /= kPieces;
+    const int which = q >= c.n_kv ? 1 : 0, head = q - which * c.n_kv;
+    const int id = page_of[r];
+    if (id < 0) continue;
     const float s = (which ? c.v_scale : c.k_scale)[kv_scale_at(c, a.layer, id, head)];
-    const int8_t* src = (which ? c.v : c.k) + kv_code_at(c, a.layer, id, head) + tok % c.page * HD + d;
+    const int8_t* src = (which ? c.v : c.k) + kv_code_at(c, a.layer, id, head) + slot_of[r] * HD + d;
     const uint4 u = *reinterpret_cast<const uint4*>(src);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     uint32_t y[8];
@@ -215,7 +244,7 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const ReadArgs a)
                                                      static_cast<float>(static_cast<int8_t>(h >> 8)) * s);
       y[e] = *reinterpret_cast<const uint32_t*>(&b);
     }
-    uint4* dst = reinterpret_cast<uint4*>(a.out[which] + row * a.ld[which] + head * HD + d);
+    uint4* dst = reinterpret_cast<uint4*>(a.out[which] + static_cast<long long>(r0 + r) * a.ld[which] + head * HD + d);
     dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
     dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
   }
@@ -236,7 +265,7 @@ extern "C" int so101_kv_append(const so101_kv_pages* c, int layer, const void* k
   if (!k || !v) return SO101_ERR_ARG;
   const int width = c->n_kv * c->hd;
   const auto a16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-  if (!a16(k) || !a16(v) || ldk % 8 || ldv % 8 || (rows > 1 && (ldk < width || ldv < width))) return SO101_ERR_ARG;
+  if (!a16(k) || !a16(v) || ldk % 8 || ldv % 8 || (cos && (!a16(cos) || !a16(sin))) || (rows > 1 && (ldk < width || ldv < width))) return SO101_ERR_ARG;
   AppendArgs a;
   a.c = *c;
   a.x[0] = static_cast<const __nv_bfloat16*>(k);

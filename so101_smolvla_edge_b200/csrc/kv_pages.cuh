@@ -53,20 +53,4 @@ __device__ __forceinline__ int kv_length(const KvPages& c, int seq, int* status)
   return len;
 }
 
-// How many of starts[0 .. n] are <= row, minus one: the sequence that holds packed row `row`
-// (starts is non-decreasing). All threads of the CTA take part; every one gets the answer. One
-// load per thread and a sum, where a binary search would chain log2(n) loads.
-__device__ __forceinline__ int find_sequence(const int* starts, int n, int row, int* shared) {
-  int below = 0;
-  for (int i = threadIdx.x; i <= n; i += blockDim.x) below += __ldg(starts + i) <= row ? 1 : 0;
-  below = __reduce_add_sync(0xffffffffu, below);
-  if (threadIdx.x == 0) *shared = 0;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0 && below) atomicAdd(shared, below);
-  __syncthreads();
-  const int at = *shared - 1;
-  __syncthreads();
-  return at;
-}
-
 }  // namespace so101
