@@ -3,14 +3,19 @@
 //   o_i = sum_{j <= i} 2^(f q_i . k_j - m_i) v_j / sum_{j <= i} 2^(f q_i . k_j - m_i),  f = scale * log2(e)
 //
 // The query heads of a kv head are stacked: row r of (sequence, kv head) is token r / group, head
-// r % group of the group, so 128 MMA rows span few tokens (43 at three heads per kv head) and little of
-// a 128-key tile is masked at the diagonal; a sequence of one token still fills `group` rows.
-// One CTA takes 128 such rows:
-//   warp 0 (one thread)  TMA: K_j and V_j (128 keys) into rings
-//   warp 1 (one thread)  S = Q K_j^T -> TMEM; O += P V_j, P read from TMEM
-//   warps 2-5            first the queries: each thread loads its row, rotates it in fp32, rounds it to
-//                        bf16 once and writes the swizzled Q tile; then the softmax of its row (one TMEM
-//                        lane), at the end O / l to the output row.
+// r % group of the group, so 128 MMA rows span few tokens (43 at three heads per kv head), little of
+// a 128-key tile is masked at the diagonal, and one K / V tile serves every head that reads it.
+// A work item is 256 such rows (two groups of 128) of one kv head. One CTA per SM walks its items, a
+// sequence's last blocks (most keys) first, in six warp groups that split the registers unevenly:
+//   0  warp 0: TMA, K_j and V_j (128 keys) into rings that run on across items
+//      warps 1, 2: the MMAs of group 0 / 1, S_g = Q_g K_j^T -> TMEM, O_g += P_g V_j, P_g read from TMEM
+//   1  the queries of the next item: loaded, rotated in fp32, rounded to bf16 into swizzled tiles
+//   2-5  the softmax, and O / l to the output rows: two threads per row (TMEM lane)
+// While a group's softmax runs, the tensor pipe works for the other one. TMEM holds S (128 columns), P and O of
+// both groups at head_dim 64; at 128, S and O only, and P takes the place of the S that it came from.
+// Rotated queries are kept in two bf16 parts at head_dim 64 (value and remainder, two MMAs into one S): tensor
+// time is not what bounds it, and the error against 64 bits falls from 2.6e-3 to 2.1e-3 (1.6e-3 is the
+// rounding of the result). At 128 there is no shared memory for the second part: one rounding to bf16.
 // The row maximum is only raised when a tile exceeds it by more than 2^8 (as in the SigLIP kernel).
 // Keys past the row's own token are masked by their index. Their values still meet P = 0 in the MMA, where an
 // infinity or a NaN in a value the row must not see would make the row NaN, so a row whose result is
@@ -30,50 +35,66 @@ struct PackedArgs {
   __nv_bfloat16* o;
   long long ldq, ldk, ldv, ldo;
   const int* starts;
-  int n_seqs, rows, group;
+  int n_seqs, rows, group, n_kv;
   const float* cos;
   const float* sin;
   float scale_log2;
   int* status;
 };
 
-constexpr int kPkRows = 128, kPkKeys = 128;
-constexpr int kPkThreads = 32 * 6;
+constexpr int kPkRows = 128;  // rows per group (MMA M)
+constexpr int kPkThreads = 768;
 constexpr float kPkStaleMax = 8.f;
+// of every 16 score pairs, how many take exp2 from the polynomial (FMA pipe) instead of MUFU
+#ifndef SO101_PACKED_POLY
+#define SO101_PACKED_POLY 3
+#endif
+constexpr int kPkPoly = SO101_PACKED_POLY;
 
-// head_dim 64: S, P and O side by side in 256 TMEM columns. 128: P takes the place of the S it came
-// from, so the next S waits for P V (the other CTA of the SM runs meanwhile).
 template <int HD>
 struct PkCfg {
-  static constexpr int kHalves = HD / 64;                 // 64-dim (128-byte) tiles of a row
-  static constexpr int kTile = kPkRows * 128;             // 16 KB: 128 rows x 64 dims
-  static constexpr int kStage = kHalves * kTile;
-  static constexpr int kStages = HD == 64 ? 2 : 1;
+  static constexpr int kHalves = HD / 64;             // 64-dim (128-byte) tiles of a row
+  static constexpr int kKeys = 128;                   // keys per tile
+  static constexpr int kQTile = kPkRows * 128;        // 16 KB: 128 rows x 64 dims
+  static constexpr int kKTile = kKeys * 128;          // kKeys rows x 64 dims
+  static constexpr int kStage = kHalves * kKTile;     // a K or V tile
+  static constexpr int kParts = HD == 64 ? 2 : 1;     // bf16 parts of a rotated query
+  static constexpr int kQBufs = HD == 64 ? 2 : 1;     // items whose queries are held
+  static constexpr int kStages = 2;                   // K and V tiles each
+  static constexpr int kQGroup = kParts * kHalves * kQTile;  // a group's queries
   static constexpr int kOffQ = 0;
-  static constexpr int kOffK = kStage;
+  static constexpr int kOffK = kQBufs * 2 * kQGroup;
   static constexpr int kOffV = kOffK + kStages * kStage;
-  static constexpr int kOffBar = kOffV + kStages * kStage;
-  static constexpr int kSmem = kOffBar + 256 + 1024;
+  static constexpr int kOffSwap = kOffV + kStages * kStage;  // [2][2 groups][2 halves][128] floats between half rows
+  static constexpr int kOffBar = kOffSwap + 4096;
+  static constexpr int kSmem = kOffBar + 768 + 1024;
+  // TMEM columns of a group. head_dim 64: S (128), P (64) and O (64) side by side; 128: S and O (128 each), P in
+  // the place of the S that it came from.
   static constexpr bool kAlias = HD == 128;
-  static constexpr uint32_t kCols = 256;
-  static constexpr uint32_t kColS = 0, kColP = kAlias ? 0 : 128, kColO = kAlias ? 128 : 192;
+  static constexpr uint32_t kColS = 0, kColP = HD == 64 ? 128 : 0, kColO = HD == 64 ? 192 : 128, kGroupCols = 256;
+  // registers per thread of the six warp groups: loads and MMAs, queries, softmax four times (480 in all, of
+  // the 80 that 768 threads start with)
+  static constexpr int kRegsLoad = 48, kRegsQuery = 48, kRegsSoft = 96;
 };
+static_assert(PkCfg<64>::kSmem <= 232448 && PkCfg<128>::kSmem <= 232448, "227 KB of shared memory per CTA");
 
 // One output row in plain fp32 over the keys it may see, by a whole warp: lane l holds dims
 // l, l + 32, ... Only for rows that came out not finite.
 template <int HD>
-__device__ __noinline__ void packed_row_alone(const PackedArgs& a, const uint8_t* q_tile, int tile_row, int start, int tok,
-                                              int kvh, long long o_at) {
+__device__ __forceinline__ void packed_row_alone(const PackedArgs& a, int start, int tok, int head, int kvh) {
   const int lane = threadIdx.x & 31;
   constexpr int N = HD / 32;
   float q[N], o[N];
+  const __nv_bfloat16* qr = a.q + (start + tok) * a.ldq + head * HD;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int d = lane + 32 * i;
-    const uint8_t* row = q_tile + (d / 64) * (kPkRows * 128) + tile_row * 128;
-    const int piece = (d % 64) / 8;
-    q[i] = __bfloat162float(
-        reinterpret_cast<const __nv_bfloat16*>(row + ((piece ^ (tile_row & 7)) << 4))[d % 8]);
+    q[i] = __bfloat162float(qr[d]);
+    if (a.cos) {
+      const long long p = static_cast<long long>(start + tok) * (HD / 2) + d % (HD / 2);
+      const float other = __bfloat162float(qr[(d + HD / 2) % HD]);
+      q[i] = d < HD / 2 ? q[i] * a.cos[p] - other * a.sin[p] : q[i] * a.cos[p] + other * a.sin[p];
+    }
     o[i] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
@@ -93,344 +114,560 @@ __device__ __noinline__ void packed_row_alone(const PackedArgs& a, const uint8_t
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = o[i] * alpha + p * __bfloat162float(vr[lane + 32 * i]);
   }
+  __nv_bfloat16* out = a.o + (start + tok) * a.ldo + head * HD;
 #pragma unroll
-  for (int i = 0; i < N; ++i) a.o[o_at + lane + 32 * i] = __float2bfloat16(l == 0.f ? 0.f : o[i] / l);
+  for (int i = 0; i < N; ++i) out[lane + 32 * i] = __float2bfloat16(l == 0.f ? 0.f : o[i] / l);
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kPkThreads, 2)
-    attention_packed_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                            const PackedArgs a) {
-  using Cfg = PkCfg<HD>;
-  constexpr int kStages = Cfg::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ int plan[4];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
-  uint64_t* q_full = bar;
-  uint64_t* k_full = bar + 1;
-  uint64_t* k_empty = k_full + kStages;
-  uint64_t* v_full = k_empty + kStages;
-  uint64_t* v_empty = v_full + kStages;
-  uint64_t* s_full = v_empty + kStages;
-  uint64_t* s_free = s_full + 1;
-  uint64_t* p_full = s_free + 1;
-  uint64_t* o_full = p_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+// A work item: rows [row_first, row_first + rows) (of the stacked ones) of the sequence that begins at packed
+// row `start`, kv head kvh. rows == 0: no more items.
+struct PackedItem {
+  int start, row_first, rows, kvh;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  grid_dep_launch();
-  grid_dep_wait();
-  // block blockIdx.x of all sequences' 128-row blocks, the sequence's last block first (most keys):
-  // warp 0 walks the sequences 32 at a time
-  if (warp == 0) {
-    int before = 0, seq = -1, start = 0, len = 0, block = 0;
-    const int want = static_cast<int>(blockIdx.x);
-    for (int s0 = 0; s0 < a.n_seqs && seq < 0; s0 += 32) {
+  // Key tiles of row group g (0: none of its rows are there).
+  __device__ __forceinline__ int tiles(const PackedArgs& a, int g, int keys) const {
+    const int here = min(rows - g * kPkRows, kPkRows);
+    return here <= 0 ? 0 : (row_first + g * kPkRows + here - 1) / a.group / keys + 1;
+  }
+  __device__ __forceinline__ int tiles(const PackedArgs& a, int keys) const { return max(tiles(a, 0, keys), tiles(a, 1, keys)); }
+};
+
+// The items of one CTA, in order, worked out by one warp for all: item w is kv head w % n_kv of block
+// w / n_kv, the blocks (256 rows) of all sequences counted in turn, each sequence's from its last, 32 sequences at a time.
+// CTA b takes item b of the first gridDim.x, the b-th last of the second, and so on in turn: items get smaller along
+// a sequence, and with the same place in every turn the first CTA would have 14% more than the average.
+struct PackedWalk {
+  int turn, s0, before;  // items taken; the window's first sequence and the blocks before it
+
+  __device__ __forceinline__ PackedItem next(const PackedArgs& a) {
+    const int lane = threadIdx.x & 31;
+    const int g = static_cast<int>(gridDim.x), b = static_cast<int>(blockIdx.x);
+    const int w = turn * g + (turn & 1 ? g - 1 - b : b);
+    ++turn;
+    const int block = w / a.n_kv;
+    PackedItem it;
+    it.kvh = w - block * a.n_kv;
+    it.start = it.row_first = it.rows = 0;
+    for (; s0 < a.n_seqs; s0 += 32) {
       const int s = s0 + lane;
-      int b = 0, at = 0, n = 0;
+      int at = 0, len = 0;
       if (s < a.n_seqs) {
         at = __ldg(a.starts + s);
-        n = __ldg(a.starts + s + 1) - at;
-        if (at < 0 || n < 0 || static_cast<long long>(at) + n > a.rows) {
+        len = __ldg(a.starts + s + 1) - at;
+        if (at < 0 || len < 0 || static_cast<long long>(at) + len > a.rows) {
           record_error(a.status, SO101_ERR_PAGES);
-          n = 0;
+          len = 0;
         }
-        b = static_cast<int>((static_cast<long long>(n) * a.group + kPkRows - 1) / kPkRows);
       }
-      int inc = b;
+      int inc = static_cast<int>((static_cast<long long>(len) * a.group + 2 * kPkRows - 1) / (2 * kPkRows));
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, inc, d);
         if (lane >= d) inc += y;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > want);
+      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > block);
       if (hit) {
-        const int w = __ffs(hit) - 1;
-        seq = s0 + w;
-        start = __shfl_sync(0xffffffffu, at, w);
-        len = __shfl_sync(0xffffffffu, n, w);
-        const int end = before + __shfl_sync(0xffffffffu, inc, w);
-        block = end - 1 - want;  // last block first
+        const int x = __ffs(hit) - 1;
+        it.start = __shfl_sync(0xffffffffu, at, x);
+        const int n = __shfl_sync(0xffffffffu, len, x);
+        it.row_first = (before + __shfl_sync(0xffffffffu, inc, x) - 1 - block) * 2 * kPkRows;
+        it.rows = min(2 * kPkRows, n * a.group - it.row_first);
+        return it;
       }
       before += __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (lane == 0) {
-      plan[0] = seq;
-      plan[1] = start;
-      plan[2] = len;
-      plan[3] = block;
-    }
+    return it;
   }
-  if (threadIdx.x == 32) {
-    mbar_init(q_full, 4);
+};
+
+constexpr int kPkItems = 8;           // items that the list in shared memory holds
+constexpr int kPkItemReaders = 25;    // reads of each: loads 1, MMAs 2 x 2 (S, P V), queries 4, softmax 16
+
+template <int HD>
+__global__ void __launch_bounds__(kPkThreads, 1)
+    attention_packed_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                            const PackedArgs a) {
+  using Cfg = PkCfg<HD>;
+  constexpr int kStages = Cfg::kStages, kQBufs = Cfg::kQBufs, kKeys = Cfg::kKeys;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  PackedItem* items = reinterpret_cast<PackedItem*>(smem + Cfg::kOffBar);
+  uint64_t* item_full = reinterpret_cast<uint64_t*>(items + kPkItems);  // [kPkItems]
+  uint64_t* item_empty = item_full + kPkItems;                         // [kPkItems] read by every warp
+  uint64_t* q_full = item_empty + kPkItems;  // [kQBufs] an item's queries are written
+  uint64_t* q_empty = q_full + kQBufs;       // [kQBufs] both groups' S MMAs have read them
+  uint64_t* k_full = q_empty + kQBufs;       // [kStages]
+  uint64_t* k_empty = k_full + kStages;      // [kStages]
+  uint64_t* v_full = k_empty + kStages;      // [kStages]
+  uint64_t* v_empty = v_full + kStages;      // [kStages]
+  uint64_t* s_full = v_empty + kStages;      // [2] per group: S written
+  uint64_t* s_free = s_full + 2;             // [2] S read into registers (head_dim 64)
+  uint64_t* p_full = s_free + 2;             // [2] P written, O rescaled
+  // [2] P V added to O; everyone waits for each of them (a phase's parity only tells it from its neighbours)
+  uint64_t* o_full = p_full + 2;
+  uint64_t* o_free = o_full + 2;             // [2] an item's O read out
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
+  static_assert(kPkItems * sizeof(PackedItem) + (2 * kPkItems + 4 + 16 + 4 + 12) * 8 + 4 <= 768, "barrier region");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPkItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], kPkItemReaders);
+    }
+    for (int i = 0; i < kQBufs; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&q_empty[i], 2);
+    }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], 2);
     }
-    mbar_init(s_full, 1);
-    mbar_init(s_free, 4);
-    mbar_init(p_full, 4);
-    mbar_init(o_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 8);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_free[i], 8);
+    }
     fence_mbar_init();
   }
-  __syncthreads();
-  if (plan[0] < 0) return;  // past the last block: nothing was allocated
-  const int start = plan[1], len = plan[2], row_first = plan[3] * kPkRows;
-  const int kvh = blockIdx.y;
-  const int rows = min(kPkRows, len * a.group - row_first);
-  const int last_tok = (row_first + rows - 1) / a.group;
-  const int n_tiles = last_tok / kPkKeys + 1;
   if (warp == 1) {
-    tmem_alloc(tmem_slot, Cfg::kCols);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  grid_dep_launch();
+  grid_dep_wait();
 
-  if (warp == 0) {
-    if (lane == 0) {
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
+  const bool parted = Cfg::kParts == 2 && a.cos != nullptr;  // a second part of the queries
+  // waits whose outcome is the same for the whole warp; the n-th use (from 0) of a barrier
+  auto wait = [&](uint64_t* b, int n) {
+    return __all_sync(0xffffffffu, mbar_wait(b, static_cast<uint32_t>(n) & 1u, a.status));
+  };
+  // item i of this CTA; rows == 0 past the last, or where a wait ran out
+  auto item_at = [&](int i) {
+    PackedItem it;
+    it.start = it.row_first = it.rows = it.kvh = 0;
+    if (wait(&item_full[i % kPkItems], i / kPkItems)) {
+      const int4 x = *reinterpret_cast<const int4*>(items + i % kPkItems);
+      it.start = x.x, it.row_first = x.y, it.rows = x.z, it.kvh = x.w;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[i % kPkItems]);
+    return it;
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsLoad));
+    if (warp == 3) {
+      // ---- the list of items
+      PackedWalk walk;
+      walk.turn = walk.s0 = walk.before = 0;
+      bool ok = true, more = true;
+      for (int i = 0; ok && more; ++i) {
+        const PackedItem it = walk.next(a);
+        more = it.rows > 0;
+        if (i >= kPkItems) ok = wait(&item_empty[i % kPkItems], i / kPkItems - 1);
+        if (ok && lane == 0) {
+          *reinterpret_cast<int4*>(items + i % kPkItems) = make_int4(it.start, it.row_first, it.rows, it.kvh);
+          mbar_arrive(&item_full[i % kPkItems]);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 0) {
+      // ---- K and V tiles
+      if (lane == 0) {
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+      }
       const uint64_t keep = policy_evict_normal();
-      for (int j = 0; j < n_tiles; ++j) {
-        const int st = j % kStages;
-        const uint32_t back = static_cast<uint32_t>(j / kStages - 1) & 1u;
-        if (j >= kStages && !mbar_wait(&k_empty[st], back, a.status)) break;
-        mbar_arrive_expect_tx(&k_full[st], Cfg::kStage);
-        for (int h = 0; h < Cfg::kHalves; ++h)
-          tma_load_2d(smem + Cfg::kOffK + st * Cfg::kStage + h * Cfg::kTile, &tm_k, &k_full[st], kvh * HD + 64 * h,
-                      start + j * kPkKeys, keep);
-        if (j >= kStages && !mbar_wait(&v_empty[st], back, a.status)) break;
-        mbar_arrive_expect_tx(&v_full[st], Cfg::kStage);
-        for (int h = 0; h < Cfg::kHalves; ++h)
-          tma_load_2d(smem + Cfg::kOffV + st * Cfg::kStage + h * Cfg::kTile, &tm_v, &v_full[st], kvh * HD + 64 * h,
-                      start + j * kPkKeys, keep);
+      int t = 0;  // this CTA's key tiles so far (ring slot and phase)
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const PackedItem it = item_at(i);
+        if (it.rows == 0) break;
+        const int n_tiles = it.tiles(a, kKeys);
+        for (int j = 0; j < n_tiles && ok; ++j, ++t) {
+          const int st = t % kStages;
+          if (t >= kStages) ok = wait(&k_empty[st], t / kStages - 1);
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(&k_full[st], Cfg::kStage);
+            for (int h = 0; h < Cfg::kHalves; ++h)
+              tma_load_2d(smem + Cfg::kOffK + st * Cfg::kStage + h * Cfg::kKTile, &tm_k, &k_full[st],
+                          it.kvh * HD + 64 * h, it.start + j * kKeys, keep);
+          }
+          if (ok && t >= kStages) ok = wait(&v_empty[st], t / kStages - 1);
+          if (ok && elect_one()) {
+            mbar_arrive_expect_tx(&v_full[st], Cfg::kStage);
+            for (int h = 0; h < Cfg::kHalves; ++h)
+              tma_load_2d(smem + Cfg::kOffV + st * Cfg::kStage + h * Cfg::kKTile, &tm_v, &v_full[st],
+                          it.kvh * HD + 64 * h, it.start + j * kKeys, keep);
+          }
+        }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t ID_S = idesc_attn(kPkKeys, 0);
+    } else {
+      // ---- the MMAs of group g, a warp each (so that neither group waits for the other's softmax),
+      // one lane elected at each issue. Two cursors walk the CTA's tiles: S runs ahead of P V by one tile,
+      // across items too.
+      const int g = warp - 1;
+      constexpr uint32_t ID_S = idesc_attn(kKeys, 0);
       constexpr uint32_t ID_O = idesc_attn(64, 1);
-      auto issue_s = [&](int j) {
-        const int st = j % kStages;
-#pragma unroll
-        for (int h = 0; h < Cfg::kHalves; ++h) {
-          const uint64_t qd = sw128_desc(smem_u32(smem + Cfg::kOffQ + h * Cfg::kTile));
-          const uint64_t kd = sw128_desc(smem_u32(smem + Cfg::kOffK + st * Cfg::kStage + h * Cfg::kTile));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_f16(tmem + Cfg::kColS, qd + 2 * k, kd + 2 * k, ID_S, h + k > 0 ? 1u : 0u);
+      const uint32_t d0 = tmem + g * Cfg::kGroupCols;
+      struct Cursor {
+        int item, j, t, mine, tiles, own;  // item, tile of it, tile of the CTA; this group's tiles of the item, all; own tiles so far
+      } cs = {-1, 0, -1, 0, 0, 0}, cp = {-1, 0, -1, 0, 0, 0};
+      int n_items = 0;  // items that this group had rows in (of the P V cursor)
+      auto pv_done = [&](int n) { return wait(&o_full[g], n); };  // this group's n-th P V
+      // To the next tile; false past the last item.
+      auto step = [&](Cursor& c) {
+        ++c.t;
+        if (c.item < 0 || ++c.j == c.tiles) {
+          ++c.item;
+          const PackedItem it = item_at(c.item);
+          c.j = 0;
+          c.mine = it.tiles(a, g, kKeys);
+          c.tiles = it.rows ? it.tiles(a, kKeys) : 0;
         }
-        mma_commit(s_full);
-        mma_commit(&k_empty[st]);
+        return c.tiles > 0;
       };
-      auto issue_pv = [&](int j) {
-        const int st = j % kStages;
+      // S of the cursor's tile (the K stage freed where the group has no rows for it)
+      auto issue_s = [&]() {
+        const int st = cs.t % kStages, qb = cs.item % kQBufs;
+        const bool has = cs.j < cs.mine;
+        if (!((cs.j > 0 || wait(&q_full[qb], cs.item / kQBufs)) && wait(&k_full[st], cs.t / kStages))) return false;
+        // the S before is in registers; where P took its place, P V has read that
+        if (has && cs.own > 0 && !(Cfg::kAlias ? pv_done(cs.own - 1) : wait(&s_free[g], cs.own - 1))) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          if (has) {
 #pragma unroll
-        for (int h = 0; h < Cfg::kHalves; ++h) {
-          const uint64_t vd = sw128_desc(smem_u32(smem + Cfg::kOffV + st * Cfg::kStage + h * Cfg::kTile));
+            for (int h = 0; h < Cfg::kHalves; ++h) {
+              const uint64_t qd = sw128_desc(smem_u32(smem + Cfg::kOffQ + (2 * qb + g) * Cfg::kQGroup + h * Cfg::kQTile));
+              const uint64_t kd = sw128_desc(smem_u32(smem + Cfg::kOffK + st * Cfg::kStage + h * Cfg::kKTile));
 #pragma unroll
-          for (int k = 0; k < kPkKeys / 16; ++k)
-            mma_f16_ta(tmem + Cfg::kColO + 64 * h, tmem + Cfg::kColP + 8 * k, vd + static_cast<uint64_t>(k) * (2048 >> 4),
-                       ID_O, (j > 0 || k > 0) ? 1u : 0u);
+              for (int k = 0; k < 4; ++k)
+                mma_f16(d0 + Cfg::kColS, qd + 2 * k, kd + 2 * k, ID_S, h + k > 0 ? 1u : 0u);
+              if (parted) {
+                const uint64_t rd = qd + (Cfg::kHalves * Cfg::kQTile >> 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_f16(d0 + Cfg::kColS, rd + 2 * k, kd + 2 * k, ID_S, 1u);
+              }
+            }
+            mma_commit(&s_full[g]);
+            mma_commit(&k_empty[st]);
+          } else {
+            mbar_arrive(&k_empty[st]);
+          }
+          if (cs.j + 1 == cs.tiles) {
+            if (has || cs.mine > 0) mma_commit(&q_empty[qb]);
+            else mbar_arrive(&q_empty[qb]);
+          }
         }
-        mma_commit(o_full);
-        mma_commit(&v_empty[st]);
+        if (has) ++cs.own;
+        return true;
       };
-      auto k_ready = [&](int j) { return mbar_wait(&k_full[j % kStages], static_cast<uint32_t>(j / kStages) & 1u, a.status); };
-      bool ok = mbar_wait(q_full, 0, a.status) && k_ready(0);
-      if (ok) {
+      auto issue_pv = [&]() {
+        const int st = cp.t % kStages;
+        const bool has = cp.j < cp.mine;
+        if (!wait(&v_full[st], cp.t / kStages) || (has && !wait(&p_full[g], cp.own))) return false;
+        if (has && cp.j == 0 && n_items > 0 && !wait(&o_free[g], n_items - 1)) return false;
         tc_fence_after();
-        issue_s(0);
-      }
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        if (!Cfg::kAlias && j + 1 < n_tiles) {  // the next S beside this tile's P V
-          ok = k_ready(j + 1) && mbar_wait(s_free, j & 1u, a.status);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(j + 1);
+        if (elect_one()) {
+          if (has) {
+            const uint32_t p = d0 + Cfg::kColP;
+#pragma unroll
+            for (int h = 0; h < Cfg::kHalves; ++h) {
+              const uint64_t vd = sw128_desc(smem_u32(smem + Cfg::kOffV + st * Cfg::kStage + h * Cfg::kKTile));
+#pragma unroll
+              for (int k = 0; k < kKeys / 16; ++k)  // 16 keys = 8 columns of P; of V, 16 rows = 2048 bytes
+                mma_f16_ta(d0 + Cfg::kColO + 64 * h, p + 8 * k, vd + static_cast<uint64_t>(k) * (2048 >> 4), ID_O,
+                           (cp.j > 0 || k > 0) ? 1u : 0u);
+            }
+            mma_commit(&o_full[g]);
+            mma_commit(&v_empty[st]);
+          } else {
+            mbar_arrive(&v_empty[st]);
+          }
         }
-        ok = mbar_wait(&v_full[j % kStages], static_cast<uint32_t>(j / kStages) & 1u, a.status) &&
-             mbar_wait(p_full, j & 1u, a.status);
-        if (!ok) break;
-        tc_fence_after();
-        issue_pv(j);
-        if (Cfg::kAlias && j + 1 < n_tiles) {  // over P, once P V (issued before it) has read it
-          ok = k_ready(j + 1);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(j + 1);
+        if (has) {
+          ++cp.own;
+          if (cp.j == 0) ++n_items;
         }
+        return true;
+      };
+      bool s_more = step(cs);
+      bool ok = s_more && issue_s();
+      if (ok) s_more = step(cs);
+      while (ok && step(cp)) {
+        // head_dim 64: the next S of the item as soon as this one is in registers, beside the softmax; then P V.
+        // 128 (where it follows P V), and another item's first S (whose queries may not be there yet): P V first
+        const bool first = !Cfg::kAlias && s_more && cs.j > 0;
+        if (first) ok = issue_s();
+        if (ok) ok = issue_pv();
+        if (ok && !first && s_more) ok = issue_s();
+        if (ok && s_more) s_more = step(cs);
       }
     }
-  } else {
-    const int quad = warp & 3;
-    const int rl = quad * 32 + lane;
-    const bool live = rl < rows;
-    const int r = row_first + (live ? rl : 0);
-    const int tok = r / a.group, head = kvh * a.group + r % a.group;
-    uint8_t* q_tile = smem + Cfg::kOffQ;
-    {
-      const __nv_bfloat16* qr = a.q + (start + tok) * a.ldq + head * HD;
-      uint4 u[HD / 8];
-#pragma unroll
-      for (int c = 0; c < HD / 8; ++c) u[c] = live ? __ldg(reinterpret_cast<const uint4*>(qr) + c) : make_uint4(0, 0, 0, 0);
+  } else if (warp < 8) {
+    // ---- the queries: 16-byte pieces copied into their swizzled places (all of an item's in flight together),
+    // then, with rotary tables, 8 dims and their partners (HD / 2 later) at a time turned in place
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsQuery));
+    constexpr int kPieces = HD / 8, kPairs = HD / 16;
+    bool ok = true;
+    for (int item = 0; ok; ++item) {
+      const PackedItem it = item_at(item);
+      if (it.rows == 0) break;
+      const int qb = item % kQBufs;
+      // a quarter of the used groups' rows per warp, padding rows as zeros
+      const int rows = (it.rows <= kPkRows ? kPkRows : 2 * kPkRows) / 4, row0 = (warp - 4) * rows;
+      const int real = min(max(it.rows - row0, 0), rows);
+      if (item >= kQBufs) ok = wait(&q_empty[qb], item / kQBufs - 1);  // the buffer's last item has been read
+      if (!ok) break;
+      uint8_t* base = smem + Cfg::kOffQ + 2 * qb * Cfg::kQGroup;
+      // piece c of row r
+      auto at = [&](int r, int c) {
+        return base + (r >= kPkRows ? Cfg::kQGroup : 0) + c / 8 * Cfg::kQTile + r % kPkRows * 128 + ((c % 8 ^ (r & 7)) << 4);
+      };
+      for (int p = lane; p < rows * kPieces; p += 32) {
+        const int r = row0 + p / kPieces, c = p % kPieces;
+        const int row = it.row_first + (r < it.rows ? r : 0), tok = row / a.group;
+        const __nv_bfloat16* src = a.q + (it.start + tok) * a.ldq + (it.kvh * a.group + row - tok * a.group) * HD + 8 * c;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at(r, c))), "l"(src),
+                     "r"(r < it.rows ? 16 : 0)
+                     : "memory");
+      }
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
       if (a.cos) {
-        const long long p = static_cast<long long>(start + tok) * (HD / 2);
+        __syncwarp();  // every lane's pieces are there
+#pragma unroll 2
+        for (int p = lane; p < real * kPairs; p += 32) {
+          const int r = row0 + p / kPairs, c = p % kPairs;
+          const long long t = static_cast<long long>(it.start + (it.row_first + r) / a.group) * (HD / 2) + 8 * c;
+          uint4* u1 = reinterpret_cast<uint4*>(at(r, c));
+          uint4* u2 = reinterpret_cast<uint4*>(at(r, c + kPairs));
+          uint4 x1 = *u1, x2 = *u2, l1, l2;
+          __nv_bfloat162* h1 = reinterpret_cast<__nv_bfloat162*>(&x1);
+          __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&x2);
+          __nv_bfloat162* r1 = reinterpret_cast<__nv_bfloat162*>(&l1);
+          __nv_bfloat162* r2 = reinterpret_cast<__nv_bfloat162*>(&l2);
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-          __nv_bfloat162* h1 = reinterpret_cast<__nv_bfloat162*>(&u[c]);
-          __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u[c + HD / 16]);
-          float cv[8], sv[8];
+          for (int e = 0; e < 4; e += 2) {
+            const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + t + 2 * e));
+            const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin + t + 2 * e));
+            const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            const float4 x = __ldg(reinterpret_cast<const float4*>(a.cos + p + 8 * c + e));
-            const float4 y = __ldg(reinterpret_cast<const float4*>(a.sin + p + 8 * c + e));
-            cv[e] = x.x, cv[e + 1] = x.y, cv[e + 2] = x.z, cv[e + 3] = x.w;
-            sv[e] = y.x, sv[e + 1] = y.y, sv[e + 2] = y.z, sv[e + 3] = y.w;
+            for (int z = 0; z < 2; ++z) {
+              const float2 v1 = __bfloat1622float2(h1[e + z]), v2 = __bfloat1622float2(h2[e + z]);
+              const float y0 = __fsub_rn(__fmul_rn(v1.x, cv[2 * z]), __fmul_rn(v2.x, sv[2 * z]));
+              const float y1 = __fsub_rn(__fmul_rn(v1.y, cv[2 * z + 1]), __fmul_rn(v2.y, sv[2 * z + 1]));
+              const float y2 = __fadd_rn(__fmul_rn(v2.x, cv[2 * z]), __fmul_rn(v1.x, sv[2 * z]));
+              const float y3 = __fadd_rn(__fmul_rn(v2.y, cv[2 * z + 1]), __fmul_rn(v1.y, sv[2 * z + 1]));
+              h1[e + z] = __floats2bfloat162_rn(y0, y1);
+              h2[e + z] = __floats2bfloat162_rn(y2, y3);
+              if (Cfg::kParts == 2) {
+                const float2 b1 = __bfloat1622float2(h1[e + z]), b2 = __bfloat1622float2(h2[e + z]);
+                r1[e + z] = __floats2bfloat162_rn(y0 - b1.x, y1 - b1.y);
+                r2[e + z] = __floats2bfloat162_rn(y2 - b2.x, y3 - b2.y);
+              }
+            }
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 x1 = __bfloat1622float2(h1[e]), x2 = __bfloat1622float2(h2[e]);
-            h1[e] = __floats2bfloat162_rn(__fsub_rn(__fmul_rn(x1.x, cv[2 * e]), __fmul_rn(x2.x, sv[2 * e])),
-                                          __fsub_rn(__fmul_rn(x1.y, cv[2 * e + 1]), __fmul_rn(x2.y, sv[2 * e + 1])));
-            h2[e] = __floats2bfloat162_rn(__fadd_rn(__fmul_rn(x2.x, cv[2 * e]), __fmul_rn(x1.x, sv[2 * e])),
-                                          __fadd_rn(__fmul_rn(x2.y, cv[2 * e + 1]), __fmul_rn(x1.y, sv[2 * e + 1])));
+          *u1 = x1;
+          *u2 = x2;
+          if (Cfg::kParts == 2) {
+            *reinterpret_cast<uint4*>(at(r, c) + Cfg::kHalves * Cfg::kQTile) = l1;
+            *reinterpret_cast<uint4*>(at(r, c + kPairs) + Cfg::kHalves * Cfg::kQTile) = l2;
           }
         }
+        if (Cfg::kParts == 2)  // the second part of padding rows
+          for (int p = real * kPieces + lane; p < rows * kPieces; p += 32)
+            *reinterpret_cast<uint4*>(at(row0 + p / kPieces, p % kPieces) + Cfg::kHalves * Cfg::kQTile) = make_uint4(0u, 0u, 0u, 0u);
       }
-#pragma unroll
-      for (int c = 0; c < HD / 8; ++c)
-        *reinterpret_cast<uint4*>(q_tile + (c / 8) * Cfg::kTile + rl * 128 + (((c % 8) ^ (rl & 7)) << 4)) = u[c];
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      if (lane == 0) mbar_arrive(&q_full[qb]);
     }
-
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t s_addr = lane_base + Cfg::kColS;
-    const uint32_t p_addr = lane_base + Cfg::kColP;
-    const uint32_t o_addr = lane_base + Cfg::kColO;
+  } else {
+    // ---- softmax of group g: row rl of its 128 (one TMEM lane) by two threads, half hf of every tile's keys
+    // each, in warps of the same scheduler. One warp alone cannot keep the exponentials' pipe busy (its
+    // instructions wait for one another), four per scheduler can.
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoft));
+    constexpr int kMine = kKeys / 2;  // keys of a tile per thread
+    const int g = (warp - 8) >> 3, hf = (warp >> 2) & 1;
+    const int quad = warp & 3;
+    const int rl = quad * 32 + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16) + g * Cfg::kGroupCols;
+    const uint32_t s_addr = lane_base + Cfg::kColS + hf * kMine, p_addr = lane_base + Cfg::kColP + hf * (kMine / 2);
+    const uint32_t o_addr = lane_base + Cfg::kColO + hf * (HD / 2);  // half of the row's O is this thread's too
+    float* swap = reinterpret_cast<float*>(smem + Cfg::kOffSwap) + g * 256 + rl;  // + 512 per buffer, 128 per half
     const float sc = a.scale_log2;
-    const int vis = live ? tok + 1 : 1;  // keys [0, vis) are visible to this row
-    float m = -INFINITY, l = 0.f;
+    auto pv_done = [&](int n) { return wait(&o_full[g], n); };  // this group's n-th P V
+    int n_swap = 0;
+    // what the other half of the row has. The two buffers take turns: a value is read before the next but one is written.
+    auto other = [&](float x) {
+      float* at = swap + (n_swap++ & 1) * 512;
+      at[hf * 128] = x;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quad) : "memory");
+      return at[(hf ^ 1) * 128];
+    };
+    int t = 0;  // this group's key tiles so far
     bool ok = true;
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      if (!mbar_wait(s_full, j & 1u, a.status)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      uint32_t sv[kPkKeys];
-#pragma unroll
-      for (int c = 0; c < kPkKeys; c += 32) tmem_ld32(s_addr + c, sv + c);
-      tmem_ld_wait();
-      if (!Cfg::kAlias) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free);
-      }
-      const int nvis = vis - j * kPkKeys;
-      if (nvis < kPkKeys) {
-#pragma unroll
-        for (int e = 0; e < kPkKeys; ++e)
-          if (e >= nvis) sv[e] = __float_as_uint(-INFINITY);
-      }
-      float mx[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) mx[t] = __uint_as_float(sv[t]);
-#pragma unroll
-      for (int e = 8; e < kPkKeys; e += 8)
-#pragma unroll
-        for (int t = 0; t < 8; ++t) mx[t] = fmaxf(mx[t], __uint_as_float(sv[e + t]));
-      const float m_tile =
-          fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * sc;
-      const bool raise = m_tile > m + kPkStaleMax;
-      const float alpha = raise ? ex2(m - m_tile) : 1.f;
-      if (raise) m = m_tile;
-      const float neg_m = m == -INFINITY ? 0.f : -m;
-      uint32_t pk[kPkKeys / 2];
-      float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < kPkKeys; e += 2) {
-        float x0, x1;
-        fma2(x0, x1, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]), sc, neg_m);
-        const float p0 = ex2(x0), p1 = ex2(x1);
-        const int t = (e >> 1) & 3;
-        add2(ls[2 * t], ls[2 * t + 1], p0, p1);
-        pk[e >> 1] = bf16x2(p0, p1);
-      }
-      const float s0 = (ls[0] + ls[2]) + (ls[4] + ls[6]), s1 = (ls[1] + ls[3]) + (ls[5] + ls[7]);
-      if (j > 0) {
-        if (!mbar_wait(o_full, (j - 1) & 1u, a.status)) {
-          ok = false;
-          break;
-        }
+    for (int item = 0; ok; ++item) {
+      const PackedItem it = item_at(item);
+      // the two warps of a row meet at every exchange, so they leave together (also after a wait ran out)
+      if (fminf(it.rows, other(it.rows)) == 0.f) break;
+      const int n_tiles = it.tiles(a, g, kKeys);
+      if (n_tiles == 0) continue;
+      const bool live = g * kPkRows + rl < it.rows;
+      const int r = it.row_first + (live ? g * kPkRows + rl : 0);
+      const int tok = r / a.group, head = it.kvh * a.group + r - tok * a.group;
+      const int vis = (live ? tok + 1 : 1) - hf * kMine;  // of its half's keys, [0, vis) are visible to this row
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n_tiles; ++j, ++t) {
+        if (ok) ok = wait(&s_full[g], t);
         tc_fence_after();
-      }
+        uint32_t sv[kMine];
 #pragma unroll
-      for (int c = 0; c < kPkKeys / 2; c += 16) tmem_st16(p_addr + c, pk + c);
-      if (j > 0 && __any_sync(0xffffffffu, raise)) {
-#pragma unroll
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t ov[32];
-          tmem_ld32(o_addr + c, ov);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-          tmem_st16(o_addr + c, ov);
-          tmem_st16(o_addr + c + 16, ov + 16);
-        }
-      }
-      l = l * alpha + (s0 + s1);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-    }
-    if (ok && mbar_wait(o_full, (n_tiles - 1) & 1u, a.status)) {
-      tc_fence_after();
-      const float inv = 1.f / l;
-      const long long o_at = (start + tok) * a.ldo + head * HD;
-      uint4* dst = reinterpret_cast<uint4*>(a.o + o_at);
-      uint32_t worst = 0u;
-#pragma unroll
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t ov[32];
-        tmem_ld32(o_addr + c, ov);
+        for (int c = 0; c < kMine; c += 32) tmem_ld32(s_addr + c, sv + c);
         tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float y = __uint_as_float(ov[e]) * inv;
-          ov[e] = __float_as_uint(y);
-          worst = max(worst, ov[e] & 0x7FFFFFFFu);
+        if (!Cfg::kAlias) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[g]);
         }
-        if (live) {
+        const int nvis = vis - j * kKeys;
+        if (nvis < kMine) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float* y = reinterpret_cast<const float*>(ov) + 8 * q;
-            dst[c / 8 + q] = make_uint4(bf16x2(y[0], y[1]), bf16x2(y[2], y[3]), bf16x2(y[4], y[5]), bf16x2(y[6], y[7]));
+          for (int e = 0; e < kMine; ++e)
+            if (e >= nvis) sv[e] = __float_as_uint(-INFINITY);
+        }
+        auto tile_max = [&]() {
+          float mx[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(sv[c]);
+#pragma unroll
+          for (int e = 4; e < kMine; e += 4)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(sv[e + c]));
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+        };
+        float m_tile = tile_max();
+        m_tile = fmaxf(m_tile, other(m_tile));  // (head_dim 128: both halves have read S, P may take its place)
+        const bool raise = m_tile > m + kPkStaleMax;
+        const float alpha = raise ? ex2(m - m_tile) : 1.f;
+        if (raise) m = m_tile;
+        const float neg_m = m == -INFINITY ? 0.f : -m;
+        float ls[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kMine; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float x0, x1, p0, p1;
+            fma2(x0, x1, __uint_as_float(sv[c + e]), __uint_as_float(sv[c + e + 1]), sc, neg_m);
+            if ((e >> 1) < kPkPoly) {
+              const float2 pp = exp2_poly2(make_float2(x0, x1));
+              p0 = pp.x, p1 = pp.y;
+            } else {
+              p0 = ex2(x0), p1 = ex2(x1);
+            }
+            const int k = (e >> 1) & 3;
+            add2(ls[2 * k], ls[2 * k + 1], p0, p1);
+            pk[e >> 1] = bf16x2(p0, p1);
+          }
+          if (c == 0 && j > 0) {  // the P V before has read P, and O is stable
+            if (ok) ok = pv_done(t - 1);
+            tc_fence_after();
+          }
+          tmem_st16(p_addr + c / 2, pk);
+        }
+        if (j > 0 && __any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int c = 0; c < HD / 2; c += 32) {
+            uint32_t ov[32];
+            tmem_ld32(o_addr + c, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+            tmem_st16(o_addr + c, ov);
+            tmem_st16(o_addr + c + 16, ov + 16);
           }
         }
+        l = l * alpha + (((ls[0] + ls[2]) + (ls[4] + ls[6])) + ((ls[1] + ls[3]) + (ls[5] + ls[7])));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
       }
-      __syncwarp();
+      l += other(l);
+      if (ok) ok = pv_done(t - 1);
+      tc_fence_after();
+      const float inv = 1.f / l;
+      uint32_t worst = 0u;
+      const long long row_at = (it.start + tok) * a.ldo + head * HD + hf * (HD / 2);
+#pragma unroll
+      for (int h = 0; h < HD / 2; h += 32) {
+        uint32_t ov[32];
+        tmem_ld32(o_addr + h, ov);
+        tmem_ld_wait();
+        if (h + 32 == HD / 2) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_free[g]);  // the next item's P V may overwrite O
+        }
+        uint4 y[4];  // 8 dims each
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[e] = __uint_as_float(ov[8 * c + e]) * inv;
+            worst = max(worst, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+          }
+          y[c] = make_uint4(bf16x2(f[0], f[1]), bf16x2(f[2], f[3]), bf16x2(f[4], f[5]), bf16x2(f[6], f[7]));
+        }
+        // 4 x 4 pieces of four lanes' rows transposed, so that a store covers eight rows of 64 bytes, not 32 of 16
+        auto swap4 = [&](uint4& lo, uint4& hi, int d) {  // the lane with bit d keeps hi, the other lo
+          const bool up = lane & d;
+          uint4 give = up ? lo : hi;
+          give.x = __shfl_xor_sync(0xffffffffu, give.x, d);
+          give.y = __shfl_xor_sync(0xffffffffu, give.y, d);
+          give.z = __shfl_xor_sync(0xffffffffu, give.z, d);
+          give.w = __shfl_xor_sync(0xffffffffu, give.w, d);
+          (up ? lo : hi) = give;
+        };
+        swap4(y[0], y[1], 1);
+        swap4(y[2], y[3], 1);
+        swap4(y[0], y[2], 2);
+        swap4(y[1], y[3], 2);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // y[c]: piece lane % 4 of row lane / 4 * 4 + c
+          const int w = (lane & ~3) + c;
+          const long long to = __shfl_sync(0xffffffffu, row_at, w);
+          if (g * kPkRows + quad * 32 + w < it.rows) *(reinterpret_cast<uint4*>(a.o + to + h) + (lane & 3)) = y[c];
+        }
+      }
+      // rows that are not finite, again (by the warp of the first half: all of the row)
+      if (!ok) worst = 0xFFFFFFFFu;
+      worst = max(worst, __float_as_uint(other(__uint_as_float(worst))));
+      if (__any_sync(0xffffffffu, worst == 0xFFFFFFFFu)) break;
       unsigned again = __ballot_sync(0xffffffffu, live && worst >= 0x7F800000u);
-      while (again) {
-        const int w = __ffs(again) - 1;
+      while (again && hf == 0) {
+        const int x = __ffs(again) - 1;
         again &= again - 1;
-        packed_row_alone<HD>(a, q_tile, quad * 32 + w, start, __shfl_sync(0xffffffffu, tok, w), kvh,
-                             __shfl_sync(0xffffffffu, o_at, w));
+        packed_row_alone<HD>(a, it.start, __shfl_sync(0xffffffffu, tok, x), __shfl_sync(0xffffffffu, head, x), it.kvh);
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, Cfg::kCols);
+  if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
 namespace {
@@ -462,16 +699,20 @@ int packed_map(CUtensorMap* m, const void* base, long long rows, long long cols,
 }
 
 template <int HD>
-int launch_packed(const CUtensorMap& tk, const CUtensorMap& tv, const PackedArgs& a, dim3 grid, cudaStream_t stream) {
-  static std::atomic<uint64_t> configured{0};  // a bit per device
+int launch_packed(const CUtensorMap& tk, const CUtensorMap& tv, const PackedArgs& a, int64_t items, cudaStream_t stream) {
+  static std::atomic<int> sms[64];
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 64 && !(configured.load() >> dev & 1)) {
-    const cudaError_t e = cudaFuncSetAttribute(attention_packed_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               PkCfg<HD>::kSmem);
+  if (dev < 0 || dev >= 64) return SO101_ERR_DRIVER;
+  int full = sms[dev].load();
+  if (!full) {
+    cudaError_t e = cudaFuncSetAttribute(attention_packed_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         PkCfg<HD>::kSmem);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&full, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return launch_error(e);
-    configured.fetch_or(1ull << dev);
+    sms[dev].store(full);
   }
+  const dim3 grid(static_cast<unsigned>(items < full ? items : full));
   return launch_kernel(attention_packed_kernel<HD>, grid, dim3(kPkThreads), PkCfg<HD>::kSmem, stream, tk, tv, a);
 }
 
@@ -517,9 +758,9 @@ extern "C" int so101_attention_packed(const void* q, int64_t ldq, const void* k,
   a.sin = sin;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = status_ptr();
-  // the blocks of all sequences: at most one part-filled block each
-  const int64_t full = rows * a.group / kPkRows;
-  const int64_t blocks = full + (n_seqs < rows ? n_seqs : rows);
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(nkv));
-  return hd == 64 ? launch_packed<64>(tk, tv, a, grid, stream) : launch_packed<128>(tk, tv, a, grid, stream);
+  a.n_kv = nkv;
+  // items: blocks of 256 rows, at most one part-filled per sequence, of every kv head
+  const int64_t items = (rows * a.group / (2 * kPkRows) + (n_seqs < rows ? n_seqs : rows)) * nkv;
+  if (items > (1 << 30)) return SO101_ERR_ARG;
+  return hd == 64 ? launch_packed<64>(tk, tv, a, items, stream) : launch_packed<128>(tk, tv, a, items, stream);
 }
