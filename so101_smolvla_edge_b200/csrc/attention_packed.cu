@@ -36,6 +36,7 @@ struct PackedArgs {
   long long ldq, ldk, ldv, ldo;
   const int* starts;
   int n_seqs, rows, group, n_kv;
+  int group_inv;  // 65536 / group + 1: x / group = x * group_inv >> 16 for x < 512
   const float* cos;
   const float* sin;
   float scale_log2;
@@ -74,7 +75,7 @@ struct PkCfg {
   static constexpr uint32_t kColS = 0, kColP = HD == 64 ? 128 : 0, kColO = HD == 64 ? 192 : 128, kGroupCols = 256;
   // registers per thread of the six warp groups: loads and MMAs, queries, softmax four times (480 in all, of
   // the 80 that 768 threads start with)
-  static constexpr int kRegsLoad = 48, kRegsQuery = 48, kRegsSoft = 96;
+  static constexpr int kRegsLoad = HD == 64 ? 40 : 48, kRegsQuery = HD == 64 ? 72 : 48, kRegsSoft = HD == 64 ? 88 : 96;
 };
 static_assert(PkCfg<64>::kSmem <= 232448 && PkCfg<128>::kSmem <= 232448, "227 KB of shared memory per CTA");
 
@@ -117,6 +118,31 @@ __device__ __forceinline__ void packed_row_alone(const PackedArgs& a, int start,
   __nv_bfloat16* out = a.o + (start + tok) * a.ldo + head * HD;
 #pragma unroll
   for (int i = 0; i < N; ++i) out[lane + 32 * i] = __float2bfloat16(l == 0.f ? 0.f : o[i] / l);
+}
+
+// Eight dims (x1) and their partners HD / 2 later (x2) of a query turned by the angles of cv / sv: each operation
+// rounded to fp32, the results to bf16, and with PARTS == 2 what that loses, in bf16 too, in l1 / l2.
+template <int PARTS>
+__device__ __forceinline__ void packed_turn(uint4& x1, uint4& x2, uint4& l1, uint4& l2, const float* cv, const float* sv) {
+  __nv_bfloat162* h1 = reinterpret_cast<__nv_bfloat162*>(&x1);
+  __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&x2);
+  __nv_bfloat162* r1 = reinterpret_cast<__nv_bfloat162*>(&l1);
+  __nv_bfloat162* r2 = reinterpret_cast<__nv_bfloat162*>(&l2);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 v1 = __bfloat1622float2(h1[e]), v2 = __bfloat1622float2(h2[e]);
+    const float y0 = __fsub_rn(__fmul_rn(v1.x, cv[2 * e]), __fmul_rn(v2.x, sv[2 * e]));
+    const float y1 = __fsub_rn(__fmul_rn(v1.y, cv[2 * e + 1]), __fmul_rn(v2.y, sv[2 * e + 1]));
+    const float y2 = __fadd_rn(__fmul_rn(v2.x, cv[2 * e]), __fmul_rn(v1.x, sv[2 * e]));
+    const float y3 = __fadd_rn(__fmul_rn(v2.y, cv[2 * e + 1]), __fmul_rn(v1.y, sv[2 * e + 1]));
+    h1[e] = __floats2bfloat162_rn(y0, y1);
+    h2[e] = __floats2bfloat162_rn(y2, y3);
+    if (PARTS == 2) {
+      const float2 b1 = __bfloat1622float2(h1[e]), b2 = __bfloat1622float2(h2[e]);
+      r1[e] = __floats2bfloat162_rn(y0 - b1.x, y1 - b1.y);
+      r2[e] = __floats2bfloat162_rn(y2 - b2.x, y3 - b2.y);
+    }
+  }
 }
 
 // A work item: rows [row_first, row_first + rows) (of the stacked ones) of the sequence that begins at packed
@@ -196,7 +222,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
   uint64_t* item_empty = item_full + kPkItems;                         // [kPkItems] read by every warp
   uint64_t* q_full = item_empty + kPkItems;  // [kQBufs] an item's queries are written
   uint64_t* q_empty = q_full + kQBufs;       // [kQBufs] both groups' S MMAs have read them
-  uint64_t* k_full = q_empty + kQBufs;       // [kStages]
+  uint64_t* q_first = q_empty + kQBufs;      // [1] the first item's queries are written
+  uint64_t* k_full = q_first + 1;            // [kStages]
   uint64_t* k_empty = k_full + kStages;      // [kStages]
   uint64_t* v_full = k_empty + kStages;      // [kStages]
   uint64_t* v_empty = v_full + kStages;      // [kStages]
@@ -210,29 +237,36 @@ __global__ void __launch_bounds__(kPkThreads, 1)
   static_assert(kPkItems * sizeof(PackedItem) + (2 * kPkItems + 4 + 16 + 4 + 12) * 8 + 4 <= 768, "barrier region");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kPkItems; ++i) {
-      mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], kPkItemReaders);
+  PackedWalk walk;  // warp 3's
+  PackedItem walked;
+  if (warp == 0) {
+    if (lane < kPkItems) {
+      mbar_init(&item_full[lane], 1);
+      mbar_init(&item_empty[lane], kPkItemReaders);
     }
-    for (int i = 0; i < kQBufs; ++i) {
-      mbar_init(&q_full[i], 4);
-      mbar_init(&q_empty[i], 2);
+    if (lane < kQBufs) {
+      mbar_init(&q_full[lane], 4);
+      mbar_init(&q_empty[lane], 2);
     }
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 2);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 2);
+    if (lane == 0) mbar_init(q_first, 16);
+    if (lane < kStages) {
+      mbar_init(&k_full[lane], 1);
+      mbar_init(&k_empty[lane], 2);
+      mbar_init(&v_full[lane], 1);
+      mbar_init(&v_empty[lane], 2);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 8);
-      mbar_init(&p_full[i], 8);
-      mbar_init(&o_full[i], 1);
-      mbar_init(&o_free[i], 8);
+    if (lane < 2) {
+      mbar_init(&s_full[lane], 1);
+      mbar_init(&s_free[lane], 8);
+      mbar_init(&p_full[lane], 8);
+      mbar_init(&o_full[lane], 1);
+      mbar_init(&o_free[lane], 8);
     }
     fence_mbar_init();
+  } else if (warp == 3) {  // the first item, beside the set-up
+    grid_dep_wait();
+    walk.turn = walk.s0 = walk.before = 0;
+    walked = walk.next(a);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -250,8 +284,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
   auto wait = [&](uint64_t* b, int n) {
     return __all_sync(0xffffffffu, mbar_wait(b, static_cast<uint32_t>(n) & 1u, a.status));
   };
-  // item i of this CTA; rows == 0 past the last, or where a wait ran out
-  auto item_at = [&](int i) {
+  // item i of this CTA; rows == 0 past the last, or where a wait ran out. Each reader takes an item once (a look
+  // does not count).
+  auto item_at = [&](int i, bool look = false) {
     PackedItem it;
     it.start = it.row_first = it.rows = it.kvh = 0;
     if (wait(&item_full[i % kPkItems], i / kPkItems)) {
@@ -259,7 +294,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       it.start = x.x, it.row_first = x.y, it.rows = x.z, it.kvh = x.w;
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&item_empty[i % kPkItems]);
+    if (lane == 0 && !look) mbar_arrive(&item_empty[i % kPkItems]);
     return it;
   };
 
@@ -267,18 +302,16 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsLoad));
     if (warp == 3) {
       // ---- the list of items
-      PackedWalk walk;
-      walk.turn = walk.s0 = walk.before = 0;
-      bool ok = true, more = true;
-      for (int i = 0; ok && more; ++i) {
-        const PackedItem it = walk.next(a);
-        more = it.rows > 0;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        if (i > 0) walked = walk.next(a);
         if (i >= kPkItems) ok = wait(&item_empty[i % kPkItems], i / kPkItems - 1);
         if (ok && lane == 0) {
-          *reinterpret_cast<int4*>(items + i % kPkItems) = make_int4(it.start, it.row_first, it.rows, it.kvh);
+          *reinterpret_cast<int4*>(items + i % kPkItems) = make_int4(walked.start, walked.row_first, walked.rows, walked.kvh);
           mbar_arrive(&item_full[i % kPkItems]);
         }
         __syncwarp();
+        if (walked.rows == 0) break;
       }
     } else if (warp == 0) {
       // ---- K and V tiles
@@ -340,7 +373,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       auto issue_s = [&]() {
         const int st = cs.t % kStages, qb = cs.item % kQBufs;
         const bool has = cs.j < cs.mine;
-        if (!((cs.j > 0 || wait(&q_full[qb], cs.item / kQBufs)) && wait(&k_full[st], cs.t / kStages))) return false;
+        // (q_full[0]'s first use is for item kQBufs)
+        const bool queries = cs.j > 0 || (cs.item == 0 ? wait(q_first, 0) : wait(&q_full[qb], cs.item / kQBufs - (qb == 0 ? 1 : 0)));
+        if (!queries || !wait(&k_full[st], cs.t / kStages)) return false;
         // the S before is in registers; where P took its place, P V has read that
         if (has && cs.own > 0 && !(Cfg::kAlias ? pv_done(cs.own - 1) : wait(&s_free[g], cs.own - 1))) return false;
         tc_fence_after();
@@ -419,8 +454,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     // then, with rotary tables, 8 dims and their partners (HD / 2 later) at a time turned in place
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsQuery));
     constexpr int kPieces = HD / 8, kPairs = HD / 16;
-    bool ok = true;
-    for (int item = 0; ok; ++item) {
+    // the softmax threads bring the first item's queries: at the start they have nothing else to do
+    bool ok = item_at(0).rows > 0;
+    for (int item = 1; ok; ++item) {
       const PackedItem it = item_at(item);
       if (it.rows == 0) break;
       const int qb = item % kQBufs;
@@ -430,63 +466,65 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       if (item >= kQBufs) ok = wait(&q_empty[qb], item / kQBufs - 1);  // the buffer's last item has been read
       if (!ok) break;
       uint8_t* base = smem + Cfg::kOffQ + 2 * qb * Cfg::kQGroup;
+      // row r of the item is token tok0 + (rem0 + r) / group, head (rem0 + r) % group
+      const int tok0 = it.start + it.row_first / a.group, rem0 = it.row_first % a.group;
+      auto token = [&](int r) { return (rem0 + r) * a.group_inv >> 16; };
       // piece c of row r
       auto at = [&](int r, int c) {
         return base + (r >= kPkRows ? Cfg::kQGroup : 0) + c / 8 * Cfg::kQTile + r % kPkRows * 128 + ((c % 8 ^ (r & 7)) << 4);
       };
+      const __nv_bfloat16* q0 = a.q + tok0 * a.ldq + it.kvh * a.group * HD;
+#pragma unroll 4
       for (int p = lane; p < rows * kPieces; p += 32) {
-        const int r = row0 + p / kPieces, c = p % kPieces;
-        const int row = it.row_first + (r < it.rows ? r : 0), tok = row / a.group;
-        const __nv_bfloat16* src = a.q + (it.start + tok) * a.ldq + (it.kvh * a.group + row - tok * a.group) * HD + 8 * c;
+        const int r = row0 + p / kPieces, c = p % kPieces, t = r < it.rows ? token(r) : 0;
+        const __nv_bfloat16* src = q0 + t * a.ldq + (r < it.rows ? rem0 + r - t * a.group : 0) * HD + 8 * c;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(at(r, c))), "l"(src),
                      "r"(r < it.rows ? 16 : 0)
                      : "memory");
       }
-      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
       if (a.cos) {
+        // a lane takes 8 dims (and their partners) of a token at a time, for all its heads; the next token's
+        // angles are asked for before this one's are used, the first ones beside the copies
+        const int first = real > 0 ? token(row0) : 0, tasks = real > 0 ? (token(row0 + real - 1) - first + 1) * kPairs : 0;
+        float4 ang[4], next[4];
+        auto ask = [&](int p, float4 (&x)[4]) {
+          if (p >= tasks) return;
+          const long long t = static_cast<long long>(tok0 + first + p / kPairs) * (HD / 2) + p % kPairs * 8;
+          x[0] = __ldg(reinterpret_cast<const float4*>(a.cos + t));
+          x[1] = __ldg(reinterpret_cast<const float4*>(a.cos + t + 4));
+          x[2] = __ldg(reinterpret_cast<const float4*>(a.sin + t));
+          x[3] = __ldg(reinterpret_cast<const float4*>(a.sin + t + 4));
+        };
+        ask(lane, next);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncwarp();  // every lane's pieces are there
-#pragma unroll 2
-        for (int p = lane; p < real * kPairs; p += 32) {
-          const int r = row0 + p / kPairs, c = p % kPairs;
-          const long long t = static_cast<long long>(it.start + (it.row_first + r) / a.group) * (HD / 2) + 8 * c;
-          uint4* u1 = reinterpret_cast<uint4*>(at(r, c));
-          uint4* u2 = reinterpret_cast<uint4*>(at(r, c + kPairs));
-          uint4 x1 = *u1, x2 = *u2, l1, l2;
-          __nv_bfloat162* h1 = reinterpret_cast<__nv_bfloat162*>(&x1);
-          __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&x2);
-          __nv_bfloat162* r1 = reinterpret_cast<__nv_bfloat162*>(&l1);
-          __nv_bfloat162* r2 = reinterpret_cast<__nv_bfloat162*>(&l2);
+        for (int p = lane; p < tasks; p += 32) {
 #pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + t + 2 * e));
-            const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin + t + 2 * e));
-            const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const float2 v1 = __bfloat1622float2(h1[e + z]), v2 = __bfloat1622float2(h2[e + z]);
-              const float y0 = __fsub_rn(__fmul_rn(v1.x, cv[2 * z]), __fmul_rn(v2.x, sv[2 * z]));
-              const float y1 = __fsub_rn(__fmul_rn(v1.y, cv[2 * z + 1]), __fmul_rn(v2.y, sv[2 * z + 1]));
-              const float y2 = __fadd_rn(__fmul_rn(v2.x, cv[2 * z]), __fmul_rn(v1.x, sv[2 * z]));
-              const float y3 = __fadd_rn(__fmul_rn(v2.y, cv[2 * z + 1]), __fmul_rn(v1.y, sv[2 * z + 1]));
-              h1[e + z] = __floats2bfloat162_rn(y0, y1);
-              h2[e + z] = __floats2bfloat162_rn(y2, y3);
-              if (Cfg::kParts == 2) {
-                const float2 b1 = __bfloat1622float2(h1[e + z]), b2 = __bfloat1622float2(h2[e + z]);
-                r1[e + z] = __floats2bfloat162_rn(y0 - b1.x, y1 - b1.y);
-                r2[e + z] = __floats2bfloat162_rn(y2 - b2.x, y3 - b2.y);
-              }
+          for (int i = 0; i < 4; ++i) ang[i] = next[i];
+          ask(p + 32, next);
+          const int c = p % kPairs, t = first + p / kPairs;
+          const int lo = max(row0, t * a.group - rem0), hi = min(row0 + real, (t + 1) * a.group - rem0);
+          const float* cv = reinterpret_cast<const float*>(ang);
+          const float* sv = cv + 8;
+          for (int r = lo; r < hi; ++r) {
+            uint4* u1 = reinterpret_cast<uint4*>(at(r, c));
+            uint4* u2 = reinterpret_cast<uint4*>(at(r, c + kPairs));
+            uint4 x1 = *u1, x2 = *u2, l1, l2;
+            packed_turn<Cfg::kParts>(x1, x2, l1, l2, cv, sv);
+            *u1 = x1;
+            *u2 = x2;
+            if (Cfg::kParts == 2) {
+              *reinterpret_cast<uint4*>(at(r, c) + Cfg::kHalves * Cfg::kQTile) = l1;
+              *reinterpret_cast<uint4*>(at(r, c + kPairs) + Cfg::kHalves * Cfg::kQTile) = l2;
             }
-          }
-          *u1 = x1;
-          *u2 = x2;
-          if (Cfg::kParts == 2) {
-            *reinterpret_cast<uint4*>(at(r, c) + Cfg::kHalves * Cfg::kQTile) = l1;
-            *reinterpret_cast<uint4*>(at(r, c + kPairs) + Cfg::kHalves * Cfg::kQTile) = l2;
           }
         }
         if (Cfg::kParts == 2)  // the second part of padding rows
           for (int p = real * kPieces + lane; p < rows * kPieces; p += 32)
             *reinterpret_cast<uint4*>(at(row0 + p / kPieces, p % kPieces) + Cfg::kHalves * Cfg::kQTile) = make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -515,6 +553,47 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quad) : "memory");
       return at[(hf ^ 1) * 128];
     };
+    {  // the first item's queries: half of row rl's pairs of pieces
+      const PackedItem it = item_at(0, true);
+      const int r = g * kPkRows + rl;
+      if (g * kPkRows < it.rows) {
+        const int row = it.row_first + (r < it.rows ? r : 0), tok = row / a.group;
+        const uint4* qr = reinterpret_cast<const uint4*>(a.q + (it.start + tok) * a.ldq +
+                                                         (it.kvh * a.group + row - tok * a.group) * HD);
+        constexpr int kPairs = HD / 16;
+        uint8_t* to = smem + Cfg::kOffQ + g * Cfg::kQGroup + rl * 128;
+#pragma unroll
+        for (int i = 0; i < kPairs / 2; ++i) {
+          const int c = hf * (kPairs / 2) + i;
+          uint4 x1 = make_uint4(0u, 0u, 0u, 0u), x2 = x1, l1 = x1, l2 = x1;
+          if (r < it.rows) {
+            x1 = __ldg(qr + c);
+            x2 = __ldg(qr + c + kPairs);
+            if (a.cos) {
+              const long long at = static_cast<long long>(it.start + tok) * (HD / 2) + 8 * c;
+              float4 ang[4];
+              ang[0] = __ldg(reinterpret_cast<const float4*>(a.cos + at));
+              ang[1] = __ldg(reinterpret_cast<const float4*>(a.cos + at + 4));
+              ang[2] = __ldg(reinterpret_cast<const float4*>(a.sin + at));
+              ang[3] = __ldg(reinterpret_cast<const float4*>(a.sin + at + 4));
+              const float* cv = reinterpret_cast<const float*>(ang);
+              packed_turn<Cfg::kParts>(x1, x2, l1, l2, cv, cv + 8);
+            }
+          }
+          uint8_t* d1 = to + c / 8 * Cfg::kQTile + ((c % 8 ^ (rl & 7)) << 4);
+          uint8_t* d2 = to + (c + kPairs) / 8 * Cfg::kQTile + (((c + kPairs) % 8 ^ (rl & 7)) << 4);
+          *reinterpret_cast<uint4*>(d1) = x1;
+          *reinterpret_cast<uint4*>(d2) = x2;
+          if (parted) {
+            *reinterpret_cast<uint4*>(d1 + Cfg::kHalves * Cfg::kQTile) = l1;
+            *reinterpret_cast<uint4*>(d2 + Cfg::kHalves * Cfg::kQTile) = l2;
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_first);
+    }
     int t = 0;  // this group's key tiles so far
     bool ok = true;
     for (int item = 0; ok; ++item) {
@@ -759,6 +838,7 @@ extern "C" int so101_attention_packed(const void* q, int64_t ldq, const void* k,
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = status_ptr();
   a.n_kv = nkv;
+  a.group_inv = 65536 / a.group + 1;
   // items: blocks of 256 rows, at most one part-filled per sequence, of every kv head
   const int64_t items = (rows * a.group / (2 * kPkRows) + (n_seqs < rows ? n_seqs : rows)) * nkv;
   if (items > (1 << 30)) return SO101_ERR_ARG;
