@@ -80,24 +80,4 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
-// 2^x for a pair, on the FMA and integer pipes instead of the MUFU unit (which the exp2 of the
-// other pairs keeps busy). x = j + f with j = rint(x) and |f| <= 1/2: adding 1.5 * 2^23 rounds x
-// to an integer held in the low mantissa bits of t; 2^f comes from a degree-3 polynomial (a
-// relative-error minimax fit on [-1/2, 1/2] made for this kernel, max relative error 7.5e-5, far
-// below the bf16 rounding P gets), and 2^j is added into its exponent field as (bits(t) << 23),
-// whose low bits are j. x is clamped to >= -126 so the exponent cannot wrap.
-__device__ __forceinline__ float2 exp2_poly2(float2 x) {
-  constexpr float kRound = 12582912.f;  // 1.5 * 2^23
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 t = fadd2(x, make_float2(kRound, kRound));
-  const float2 r = fadd2(t, make_float2(-kRound, -kRound));
-  const float2 f = fadd2(x, make_float2(-r.x, -r.y));
-  float2 q = ffma2(make_float2(5.517161265e-02f, 5.517161265e-02f), f, make_float2(2.426111251e-01f, 2.426111251e-01f));
-  q = ffma2(q, f, make_float2(6.932609677e-01f, 6.932609677e-01f));
-  q = ffma2(q, f, make_float2(9.999280572e-01f, 9.999280572e-01f));
-  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(t.y) << 23)));
-}
-
 }  // namespace so101
