@@ -45,7 +45,6 @@ struct PackedArgs {
 };
 
 constexpr int kPkRows = 128;  // rows per group (MMA M)
-constexpr int kPkThreads = 768;
 constexpr float kPkStaleMax = 8.f;
 template <int HD>
 struct PkCfg {
@@ -68,9 +67,12 @@ struct PkCfg {
   // the place of the S that it came from.
   static constexpr bool kAlias = HD == 128;
   static constexpr uint32_t kColS = 0, kColP = HD == 64 ? 128 : 0, kColO = HD == 64 ? 192 : 128, kGroupCols = 256;
-  // registers per thread of the six warp groups: loads and MMAs, queries, softmax four times (480 in all, of
-  // the 80 that 768 threads start with)
+  // Warps: four for loads, MMAs and the item list, then the queries', then 16 for the softmax. Registers per thread
+  // of each kind: together no more than the threads start with (80 of 768 threads).
+  static constexpr int kQWarps = 4;
+  static constexpr int kThreads = 32 * (4 + kQWarps + 16);
   static constexpr int kRegsLoad = HD == 64 ? 40 : 48, kRegsQuery = HD == 64 ? 72 : 48, kRegsSoft = HD == 64 ? 88 : 96;
+  static constexpr int kItemReaders = 1 + 4 + kQWarps + 16;  // reads of each item: loads, MMAs 2 x 2 (S, P V), queries, softmax
 };
 static_assert(PkCfg<64>::kSmem <= 232448 && PkCfg<128>::kSmem <= 232448, "227 KB of shared memory per CTA");
 
@@ -209,10 +211,9 @@ struct PackedWalk {
 };
 
 constexpr int kPkItems = 8;           // items that the list in shared memory holds
-constexpr int kPkItemReaders = 25;    // reads of each: loads 1, MMAs 2 x 2 (S, P V), queries 4, softmax 16
 
 template <int HD>
-__global__ void __launch_bounds__(kPkThreads, 1)
+__global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
     attention_packed_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                             const PackedArgs a) {
   using Cfg = PkCfg<HD>;
@@ -244,10 +245,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
   if (warp == 0) {
     if (lane < kPkItems) {
       mbar_init(&item_full[lane], 1);
-      mbar_init(&item_empty[lane], kPkItemReaders);
+      mbar_init(&item_empty[lane], Cfg::kItemReaders);
     }
     if (lane < kQBufs) {
-      mbar_init(&q_full[lane], 4);
+      mbar_init(&q_full[lane], Cfg::kQWarps);
       mbar_init(&q_empty[lane], 2);
     }
     if (lane == 0) mbar_init(q_first, 16);
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         if (ok && s_more) s_more = step(cs);
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < 4 + Cfg::kQWarps) {
     // ---- the queries: 16-byte pieces copied into their swizzled places (all of an item's in flight together),
     // then, with rotary tables, 8 dims and their partners (HD / 2 later) at a time turned in place
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsQuery));
@@ -462,8 +463,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       const PackedItem it = item_at(item);
       if (it.rows == 0) break;
       const int qb = item % kQBufs;
-      // a quarter of the used groups' rows per warp, padding rows as zeros
-      const int rows = (it.rows <= kPkRows ? kPkRows : 2 * kPkRows) / 4, row0 = (warp - 4) * rows;
+      // the used groups' rows shared out to the warps, padding rows as zeros
+      const int rows = (it.rows <= kPkRows ? kPkRows : 2 * kPkRows) / Cfg::kQWarps, row0 = (warp - 4) * rows;
       const int real = min(max(it.rows - row0, 0), rows);
       if (item >= kQBufs) ok = wait(&q_empty[qb], item / kQBufs - 1);  // the buffer's last item has been read
       if (!ok) break;
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     // instructions wait for one another), four per scheduler can.
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoft));
     constexpr int kMine = kKeys / 2;  // keys of a tile per thread
-    const int g = (warp - 8) >> 3, hf = (warp >> 2) & 1;
+    const int g = (warp - 4 - Cfg::kQWarps) >> 3, hf = (warp >> 2) & 1;
     const int quad = warp & 3;
     const int rl = quad * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16) + g * Cfg::kGroupCols;
@@ -799,7 +800,7 @@ int launch_packed(const CUtensorMap& tk, const CUtensorMap& tv, PackedArgs a, cu
   const int64_t items = (stacked / a.block + part) * a.n_kv;
   if (items > (1 << 30)) return SO101_ERR_ARG;
   const dim3 grid(static_cast<unsigned>(items < full ? items : full));
-  return launch_kernel(attention_packed_kernel<HD>, grid, dim3(kPkThreads), PkCfg<HD>::kSmem, stream, tk, tv, a);
+  return launch_kernel(attention_packed_kernel<HD>, grid, dim3(PkCfg<HD>::kThreads), PkCfg<HD>::kSmem, stream, tk, tv, a);
 }
 
 }  // namespace

@@ -63,6 +63,9 @@ struct PgCfg {
   static constexpr int kStep = kRings * kKeys;         // keys that the CTA takes at a time
   static constexpr int kTile = kKeys * HD;
   static constexpr int kStages = kRings == 4 ? 2 : 4;
+  // tiles asked for ahead: where several warps read a ring, a stage is filled again only a tile's work after its
+  // own, so that they need not run in step
+  static constexpr int kAhead = kRowWarps == 1 ? kStages - 1 : kStages - 2;
   static constexpr int kMaxPages = kKeys / 16;
   static constexpr int kRing = kStages * 2 * kTile;
   static constexpr int kSlot = ROWS * (HD + 2);        // floats of a part: its rows of O, then their (m, l)
@@ -70,7 +73,7 @@ struct PgCfg {
   static constexpr int kJoin = kPgWarps * 16 * (kJoinRow + 2) * 4;  // the rings' buffers serve the join too
   static constexpr int kOffScale = kRings * kRing > kJoin ? kRings * kRing : kJoin;
   static constexpr int kOffBar = kOffScale + kRings * kStages * 2 * kMaxPages * 4;
-  static constexpr int kOffPlan = kOffBar + kRings * kStages * 8;
+  static constexpr int kOffPlan = kOffBar + 2 * kRings * kStages * 8;
   static constexpr int kSmem = kOffPlan + 64;
 };
 
@@ -218,9 +221,11 @@ __device__ __forceinline__ PagesPlan pages_plan(const PagesArgs& a, int* shared)
   return p;
 }
 
-// GRAN: slots of a page that a tile holds (a tile is one page, several, or a part of one).
+// GRAN: slots of a page that a tile holds (a tile is one page, several, or a part of one). Three CTAs per SM (four of the
+// 64-row kernel of head_dim 64) at the price of a few spilled registers: 64 chunks of 50 tokens over 291 keys take
+// 46 us, 57 with two.
 template <int HD, int ROWS, int GRAN>
-__global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_pages_kernel(const PagesArgs a) {
+__global__ void __launch_bounds__(kPgThreads, HD == 64 && ROWS == 64 ? 4 : 3) attention_pages_kernel(const PagesArgs a) {
   using Cfg = PgCfg<HD, ROWS>;
   constexpr int kKeys = Cfg::kKeys, kStages = Cfg::kStages, kTile = Cfg::kTile;
   constexpr int kRings = Cfg::kRings, kRowWarps = Cfg::kRowWarps;
@@ -238,7 +243,10 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
   const KvPages& c = a.c;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kRings * kStages; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < kRings * kStages; ++i) {
+      mbar_init(&bars[i], kRowWarps == 1 ? 1 : 2);  // the copies (and, for other warps, the scales)
+      mbar_init(&bars[kRings * kStages + i], kRowWarps);  // read by every warp of the ring
+    }
     fence_mbar_init();
   }
   grid_dep_launch();
@@ -249,13 +257,9 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
   uint8_t* my_ring = smem + ring * Cfg::kRing;
   float* my_scales = reinterpret_cast<float*>(smem + Cfg::kOffScale) + ring * kStages * 2 * Cfg::kMaxPages;
   uint64_t* my_bars = bars + ring * kStages;
+  uint64_t* my_empty = my_bars + kRings * kStages;
   const int page_log2 = __ffs(c.page) - 1;
   constexpr int per_tile = kKeys / GRAN;  // copies of K (and of V) per tile
-  auto ring_sync = [&]() {  // the warps that read one ring
-    if (kRowWarps == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(1 + ring), "r"(32 * kRowWarps) : "memory");
-  };
-
   int entry = plan.entry, entry_first = plan.first;
   int at = plan.begin;  // the next step of this CTA's run
   int used = 0;         // tiles that this ring has taken (stages and phases)
@@ -312,7 +316,10 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
     };
     float k_sc = 0.f, v_sc = 0.f;
     auto issue = [&](int i, int id) {
-      const int key = run_key(i), st = (used + i) % kStages;
+      const int n = used + i, key = run_key(i), st = n % kStages;
+      if (kRowWarps > 1 && n >= kStages)
+        ok = __all_sync(0xffffffffu, mbar_wait(&my_empty[st], static_cast<uint32_t>(n / kStages - 1) & 1u, a.status));
+      if (!ok) return;
       bool mine = lane < per_tile && key < key1;
       if (mine && (id < 0 || id >= c.n_pages)) {
         record_error(a.status, SO101_ERR_PAGES);
@@ -340,15 +347,17 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
         my_scales[st * 2 * Cfg::kMaxPages + lane] = k_sc;
         my_scales[st * 2 * Cfg::kMaxPages + Cfg::kMaxPages + lane] = v_sc;
       }
+      __syncwarp();
+      if (kRowWarps > 1 && lane == 0) mbar_arrive(&my_bars[st]);
     };
     int next_id = -1;
     if (roww == 0) {
       next_id = page_of(0);
-      for (int i = 0; i < kStages - 1 && i < tiles; ++i) {
+      for (int i = 0; i < Cfg::kAhead && i < tiles; ++i) {
         const int id = next_id;
         next_id = page_of(i + 1);
         if (ok) issue(i, id);
-        put_scales(i);
+        if (ok) put_scales(i);
       }
     }
 
@@ -441,7 +450,6 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
 #pragma unroll
       for (int i = 0; i < kHalfRows; ++i) q_sum[i] = sums[2 * i] * 128.f * kCode;
     }
-    ring_sync();
 
     float o[kHalves][8][4];
 #pragma unroll
@@ -454,19 +462,19 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
 
     for (int i = 0; i < tiles; ++i) {
       const int st = (used + i) % kStages;
-      const bool more = ok && roww == 0 && i + kStages - 1 < tiles;
+      const bool more = ok && roww == 0 && i + Cfg::kAhead < tiles;
       if (more) {
         const int id = next_id;
-        next_id = page_of(i + kStages);
-        issue(i + kStages - 1, id);
+        next_id = page_of(i + Cfg::kAhead + 1);
+        issue(i + Cfg::kAhead, id);
       }
-      // after a wait that ran out the loop goes on without loads or waits, so that the warps of a ring
-      // still meet; the result is void and the status word says so
+      // after a wait that ran out the loop goes on without loads or waits, so that the CTA's warps still
+      // meet; the result is void and the status word says so
       if (ok) ok = mbar_wait(&my_bars[st], static_cast<uint32_t>((used + i) / kStages) & 1u, a.status);
       ok = __all_sync(0xffffffffu, ok);
       if (wrow >= rows) {  // padding rows only
-        if (more) put_scales(i + kStages - 1);
-        ring_sync();
+        if (more && ok) put_scales(i + Cfg::kAhead);
+        if (kRowWarps > 1 && lane == 0) mbar_arrive(&my_empty[st]);
         continue;
       }
       const uint8_t* kt = my_ring + st * 2 * kTile;
@@ -495,8 +503,14 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
         const float sk = ks[8 * j / GRAN];
+        float mul[2], add[2];  // (S - q_sum) * factor * scale
 #pragma unroll
-        for (int e = 0; e < 2 * kHalfRows; ++e) s[j][e] = (s[j][e] - q_sum[e >> 1]) * (sk * factor[e >> 1]);
+        for (int r = 0; r < kHalfRows; ++r) {
+          mul[r] = sk * factor[r];
+          add[r] = -q_sum[r] * mul[r];
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * kHalfRows; ++e) s[j][e] = fmaf(s[j][e], mul[e >> 1], add[e >> 1]);
       }
       if (__any_sync(0xffffffffu, tile_key + kKeys > vis_low)) {
 #pragma unroll
@@ -580,8 +594,9 @@ __global__ void __launch_bounds__(kPgThreads, ROWS <= 16 ? 3 : 2) attention_page
           }
         }
       }
-      if (more) put_scales(i + kStages - 1);
-      ring_sync();  // the stage is read: the next load may fill it
+      if (more && ok) put_scales(i + Cfg::kAhead);
+      __syncwarp();  // the stage is read: a later load may fill it
+      if (kRowWarps > 1 && lane == 0) mbar_arrive(&my_empty[st]);
     }
     if (!ok && roww == 0)  // copies in flight land before the ring's memory is used otherwise
       for (int n = max(0, issued - kStages); n < issued; ++n)
