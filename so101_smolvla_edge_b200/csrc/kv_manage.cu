@@ -4,8 +4,7 @@
 // All on the device, so that a serving loop neither waits for the GPU nor mirrors its tables. One CTA
 // orders what has to be ordered (free pages by number, list entries by place) with prefix sums: the
 // same inputs give the same pages, and a call that cannot be met changes nothing. Fork and compact leave
-// a list of page moves in the scratch ints, which all CTAs of the same launch then carry out: the CTA that
-// arrives first plans, the others wait (bounded) for its flag. A page is n_layers x 2 runs of
+// a list of page moves, which all CTAs of the same launch carry out. A page is n_layers x 2 runs of
 // n_kv * page * hd bytes (20 KB for five heads of 64 and 64 slots); the runs go through shared
 // memory in bulk copies, eight in flight per SM, bounded by the HBM copy rate.
 #include <atomic>
@@ -18,7 +17,7 @@ constexpr int kPlanThreads = 512;
 
 // Scratch ints: number of moves, arrivals, the plan's flag and departures (the last three zero between
 // calls), then src[most], dst[most] (most = max(n_pages, max_seqs)), then
-// remap[n_pages] and the parents' lengths / running offsets [max_seqs].
+// remap[n_pages], and per list entry running offsets or parents' lengths [max_seqs] and places [max_seqs].
 struct Scratch {
   int* moves;
   int* arrived;
@@ -28,6 +27,7 @@ struct Scratch {
   int* dst;
   int* remap;
   int* aux;
+  int* place;
 };
 
 __host__ __device__ inline long long scratch_most(const KvPages& c) { return c.n_pages > c.max_seqs ? c.n_pages : c.max_seqs; }
@@ -43,6 +43,7 @@ __device__ __forceinline__ Scratch scratch_of(const KvPages& c) {
   s.dst = s.src + most;
   s.remap = s.dst + most;
   s.aux = s.remap + c.n_pages;
+  s.place = s.aux + c.max_seqs;
   return s;
 }
 
@@ -176,16 +177,21 @@ __global__ void __launch_bounds__(kFreeThreads) kv_free_kernel(const ListArgs g)
   }
 }
 
-__device__ __forceinline__ void plan_fork(const ListArgs& g, int* warp_sums) {
+// What a fork or a compaction moves, worked out from the cache as it stands, nothing changed: page src[k] to page
+// dst[k]. For a fork also each entry's parent length and its place among the copies (-1: none).
+struct MovePlan {
+  int* src;
+  int* dst;
+  int* len;
+  int* place;
+};
+
+// The number of copies; -1 where the call cannot be met. Whole CTA.
+__device__ __forceinline__ int plan_fork(const ListArgs& g, const MovePlan& m, int* warp_sums) {
   __shared__ int bad;
   const KvPages& c = g.c;
-  const Scratch s = scratch_of(c);
-  if (threadIdx.x == 0) {
-    bad = 0;
-    *s.moves = 0;
-  }
+  if (threadIdx.x == 0) bad = 0;
   __syncthreads();
-  // entry i: its parent's length into aux, its place among the copies kept beside it (remap)
   int copies = 0;
   for (int i0 = 0; i0 < g.n; i0 += kPlanThreads) {
     const int i = i0 + static_cast<int>(threadIdx.x);
@@ -198,23 +204,24 @@ __device__ __forceinline__ void plan_fork(const ListArgs& g, int* warp_sums) {
         len = 0;
       }
       part = len % c.page ? 1 : 0;
-      s.aux[i] = len;
+      m.len[i] = len;
     }
     int here;
-    const int off = block_scan(part, here, warp_sums);
-    if (i < g.n) s.dst[i] = copies + off;
+    const int off = copies + block_scan(part, here, warp_sums);
+    if (i < g.n) m.place[i] = part ? off : -1;
+    if (part) m.src[off] = c.table[static_cast<long long>(g.a[i]) * c.max_pages + len / c.page];
     copies += here;
   }
   __syncthreads();
-  // the fresh pages, listed where the remap of a compaction would be
-  const bool enough = !bad && copies <= c.n_pages && free_pages(c, copies, s.remap, warp_sums);
-  if (!enough) {
-    if (threadIdx.x == 0) record_error(g.status, SO101_ERR_PAGES);
-    return;
-  }
-  for (int i = threadIdx.x >> 5; i < g.n; i += kPlanThreads / 32) {  // a warp per entry
-    const int lane = threadIdx.x & 31;
-    const int par = g.a[i], chi = g.b[i], len = s.aux[i], whole = len / c.page;
+  return !bad && copies <= c.n_pages && free_pages(c, copies, m.dst, warp_sums) ? copies : -1;
+}
+
+// The bookkeeping of a planned fork, a warp per entry, by warps [first, first + warps) of the CTA.
+__device__ __forceinline__ void apply_fork(const ListArgs& g, const MovePlan& m, int first, int warps) {
+  const KvPages& c = g.c;
+  const int lane = threadIdx.x & 31;
+  for (int i = static_cast<int>(threadIdx.x >> 5) - first; i < g.n; i += warps) {
+    const int par = g.a[i], chi = g.b[i], len = m.len[i], whole = len / c.page, place = m.place[i];
     const int* from = c.table + static_cast<long long>(par) * c.max_pages;
     int* to = c.table + static_cast<long long>(chi) * c.max_pages;
     for (int j = lane; j < c.max_pages; j += 32) {
@@ -223,10 +230,8 @@ __device__ __forceinline__ void plan_fork(const ListArgs& g, int* warp_sums) {
         id = from[j];
         if (id >= 0 && id < c.n_pages) atomicAdd(c.refs + id, 1);
         else record_error(g.status, SO101_ERR_PAGES);
-      } else if (j == whole && len % c.page) {
-        const int k = s.dst[i];
-        id = s.remap[k];
-        s.src[k] = from[j];
+      } else if (j == whole && place >= 0) {
+        id = m.dst[place];
         c.refs[id] = 1;
       }
       if (par != chi) to[j] = id;
@@ -234,15 +239,11 @@ __device__ __forceinline__ void plan_fork(const ListArgs& g, int* warp_sums) {
     __syncwarp();
     if (lane == 0) c.lengths[chi] = len;
   }
-  __syncthreads();
-  for (int k = threadIdx.x; k < copies; k += kPlanThreads) s.dst[k] = s.remap[k];
-  if (threadIdx.x == 0) *s.moves = copies;
 }
 
-// Live pages past the live count into the free ones below it, both ascending.
-__device__ __forceinline__ void plan_compact(const ListArgs& g, int* warp_sums) {
+// Live pages past the live count into the free ones below it, both ascending: how many. Whole CTA.
+__device__ __forceinline__ int plan_compact(const ListArgs& g, const MovePlan& m, int* warp_sums) {
   const KvPages& c = g.c;
-  const Scratch s = scratch_of(c);
   int live = 0;
   for (int p = threadIdx.x; p < c.n_pages; p += kPlanThreads) live += c.refs[p] > 0 ? 1 : 0;
   int total;
@@ -250,25 +251,33 @@ __device__ __forceinline__ void plan_compact(const ListArgs& g, int* warp_sums) 
   int high = 0, holes = 0;
   for (int p0 = 0; p0 < c.n_pages; p0 += kPlanThreads) {
     const int p = p0 + static_cast<int>(threadIdx.x);
-    const bool in = p < c.n_pages;
-    const bool used = in && c.refs[p] > 0;
-    const int move = used && p >= total, hole = in && !used && p < total;
+    const bool used = p < c.n_pages && c.refs[p] > 0;
+    const int move = used && p >= total, hole = p < c.n_pages && !used && p < total;
     int sum;  // both counts in one scan: at most 512 of each per turn
     const int off = block_scan(move | hole << 16, sum, warp_sums);
-    if (move) s.src[high + (off & 0xFFFF)] = p;
-    if (hole) s.dst[holes + (off >> 16)] = p;
-    if (in) s.remap[p] = p;
+    if (move) m.src[high + (off & 0xFFFF)] = p;
+    if (hole) m.dst[holes + (off >> 16)] = p;
     high += sum & 0xFFFF;
     holes += sum >> 16;
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < high; k += kPlanThreads) {
-    const int from = s.src[k], to = s.dst[k];
-    s.remap[from] = to;
+  return high;
+}
+
+// The counts of a planned compaction, and every page's new number into remap (-> the tables), by the threads
+// from `first` on, which meet at named barrier 1.
+__device__ __forceinline__ void apply_compact(const ListArgs& g, const MovePlan& m, int moves, int* remap, int first) {
+  const KvPages& c = g.c;
+  const int t = static_cast<int>(threadIdx.x) - first, step = kPlanThreads - first;
+  for (int p = t; p < c.n_pages; p += step) remap[p] = p;
+  asm volatile("bar.sync 1, %0;" ::"r"(step) : "memory");
+  for (int k = t; k < moves; k += step) {
+    const int from = m.src[k], to = m.dst[k];
+    remap[from] = to;
     c.refs[to] = c.refs[from];
     c.refs[from] = 0;
   }
-  if (threadIdx.x == 0) *s.moves = high;
+  asm volatile("bar.sync 1, %0;" ::"r"(step) : "memory");
 }
 
 enum { kMoveCopy, kMoveFork, kMoveCompact };
@@ -277,8 +286,12 @@ constexpr int kMoveChunk = 16384;  // bytes of a run that go at once, at most
 
 constexpr int kMoveBatch = 512;  // units whose addresses the CTA works out together
 
+constexpr int kSmallList = 4096;   // moves and fork entries that a plan in shared memory holds
+constexpr int kSmallTable = 16384;  // table entries that one CTA rewrites
+
 struct MoveSmem {
   uint8_t data[kMoveStages][kMoveChunk];
+  int src[kSmallList], dst[kSmallList], len[kSmallList], place[kSmallList];
   const int8_t* from[kMoveBatch];
   int8_t* to[kMoveBatch];
   int bytes[kMoveBatch];  // 0: a page out of range
@@ -305,11 +318,15 @@ __device__ __forceinline__ void st_release(int* p, int v) {
   asm volatile("st.release.gpu.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
 
-// Plan (fork, compact), then move. Unit u of the moves is (move, layer, keys or values, chunk); CTA b
+// Plan (fork, compact), then move. SMALL: every CTA works the plan out for itself, in shared memory, and starts to
+// copy; the CTA that is last to have done so (an atomic count) then changes the bookkeeping, beside its copies, so
+// that nobody waits. Larger lists and tables: the first CTA to arrive plans for all, in the scratch ints, the
+// others wait (bounded) for its flag. (The flag cost a fork of 64 and a compaction of 20 MB 4 us each.)
+// Unit u of the moves is (move, layer, keys or values, chunk); CTA b
 // takes units b, b + gridDim.x, ...: all its threads work out the addresses of a batch of them (a single
 // thread that looks each page number up itself moves a unit in 2 us: 266 us for 335 MB), then
 // thread 0 keeps kMoveStages / 2 loads ahead of the stores.
-template <int MODE>
+template <int MODE, bool SMALL>
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs g) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   MoveSmem& sm = *reinterpret_cast<MoveSmem*>(smem_raw);
@@ -323,15 +340,41 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs
   }
   grid_dep_launch();
   grid_dep_wait();
-  if (MODE != kMoveCopy) {
+  int moves = g.n;
+  bool settle = false;   // this CTA changes the bookkeeping
+  bool planned = true;
+  MovePlan m = {s.src, s.dst, s.aux, s.place};
+  if (SMALL) m = {sm.src, sm.dst, sm.len, sm.place};
+  if (MODE != kMoveCopy && SMALL) {
+    __syncthreads();
+    moves = MODE == kMoveFork ? plan_fork(g, m, warp_sums) : plan_compact(g, m, warp_sums);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      shared = atomicAdd(s.left, 1) == static_cast<int>(gridDim.x) - 1;
+      if (shared) *s.left = 0;
+      __threadfence();
+    }
+    __syncthreads();
+    settle = shared;
+    if (moves < 0) {
+      if (settle && threadIdx.x == 0) record_error(g.status, SO101_ERR_PAGES);
+      return;
+    }
+  } else if (MODE != kMoveCopy) {
     // the first CTA to arrive plans: it is running, so the others may wait for it
     if (threadIdx.x == 0) shared = atomicAdd(s.arrived, 1);
     __syncthreads();
     if (shared == 0) {
-      if (MODE == kMoveFork) plan_fork(g, warp_sums);
-      else plan_compact(g, warp_sums);
+      moves = MODE == kMoveFork ? plan_fork(g, m, warp_sums) : plan_compact(g, m, warp_sums);
+      if (moves >= 0) {
+        if (MODE == kMoveFork) apply_fork(g, m, 0, kPlanThreads / 32);
+        else apply_compact(g, m, moves, s.remap, 0);
+      }
       __syncthreads();
       if (threadIdx.x == 0) {
+        if (moves < 0) record_error(g.status, SO101_ERR_PAGES);
+        *s.moves = max(moves, 0);
         __threadfence();
         st_release(s.ready, 1);
       }
@@ -342,15 +385,16 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs
           record_error(g.status, SO101_ERR_TIMEOUT);
           break;
         }
-        __nanosleep(100);
+        __nanosleep(50);
       }
     }
     __syncthreads();
+    planned = ld_acquire(s.ready);
+    moves = planned ? __ldcg(s.moves) : 0;
   }
-  const bool planned = MODE == kMoveCopy || ld_acquire(s.ready);
-  const int* src = MODE == kMoveCopy ? g.a : s.src;
-  const int* dst = MODE == kMoveCopy ? g.b : s.dst;
-  const int moves = MODE == kMoveCopy ? g.n : planned ? __ldcg(s.moves) : 0;
+  // a move's pages: from the caller's lists, the CTA's own, or the scratch ints that another SM wrote
+  auto src_of = [&](int k) { return MODE == kMoveCopy ? g.a[k] : SMALL ? sm.src[k] : __ldcg(s.src + k); };
+  auto dst_of = [&](int k) { return MODE == kMoveCopy ? g.b[k] : SMALL ? sm.dst[k] : __ldcg(s.dst + k); };
   const int run = c.n_kv * c.page * c.hd;  // bytes per move, layer, keys or values
   const int chunks = (run + kMoveChunk - 1) / kMoveChunk;
   const int chunk = ((run + chunks - 1) / chunks + 15) / 16 * 16;
@@ -365,15 +409,17 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs
       const int h = static_cast<int>((e >> 1) % c.n_kv);
       const long long w = (e >> 1) / c.n_kv;
       const int layer = static_cast<int>(w % c.n_layers), k = static_cast<int>(w / c.n_layers);
-      const int from = __ldcg(src + k), to = __ldcg(dst + k);
+      const int from = src_of(k), to = dst_of(k);
       if (from < 0 || from >= c.n_pages || to < 0 || to >= c.n_pages) continue;
       float* sc = which ? c.v_scale : c.k_scale;
       sc[kv_scale_at(c, layer, to, h)] = sc[kv_scale_at(c, layer, from, h)];
     }
-    if (MODE == kMoveCompact && planned) {
+    if (MODE == kMoveFork && SMALL && settle) apply_fork(g, m, 1, kPlanThreads / 32 - 1);
+    if (MODE == kMoveCompact && (SMALL ? settle : planned)) {
+      if (SMALL) apply_compact(g, m, moves, s.remap, 32);
       const long long entries = static_cast<long long>(c.max_seqs) * c.max_pages;
-      for (long long e = static_cast<long long>(blockIdx.x) * step + t; e < entries;
-           e += static_cast<long long>(gridDim.x) * step) {
+      const long long at = SMALL ? t : static_cast<long long>(blockIdx.x) * step + t;
+      for (long long e = at; e < entries; e += SMALL ? step : static_cast<long long>(gridDim.x) * step) {
         const int id = c.table[e];
         if (id >= 0 && id < c.n_pages) c.table[e] = __ldcg(s.remap + id);
       }
@@ -389,7 +435,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs
       const long long u = blockIdx.x + (i0 + i) * gridDim.x, w = u / chunks;
       const int off = static_cast<int>(u % chunks) * chunk;
       const int layer = static_cast<int>((w >> 1) % c.n_layers), k = static_cast<int>((w >> 1) / c.n_layers);
-      const int from = __ldcg(src + k), to = __ldcg(dst + k);
+      const int from = src_of(k), to = dst_of(k);
       const bool valid = from >= 0 && from < c.n_pages && to >= 0 && to < c.n_pages;
       if (!valid) record_error(g.status, SO101_ERR_PAGES);
       int8_t* codes = (w & 1) ? c.v : c.k;
@@ -426,7 +472,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs
     }
   }
   if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  if (MODE != kMoveCopy) {
+  if (MODE != kMoveCopy && !SMALL) {
     __syncthreads();
     if (threadIdx.x == 0 && atomicAdd(s.left, 1) == static_cast<int>(gridDim.x) - 1) {
       *s.arrived = 0;
@@ -449,15 +495,15 @@ ListArgs list_args(const KvPages* c, const int* a, const int* b, int n) {
 }
 
 // At most `most` moves (an upper bound is enough: the list's own length rules), one CTA per SM.
-template <int MODE>
-int move_pages(const ListArgs& g, long long most, cudaStream_t stream) {
+template <int MODE, bool SMALL>
+int launch_moves(const ListArgs& g, long long most, cudaStream_t stream) {
   static std::atomic<int> sms[64];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return SO101_ERR_DRIVER;
   int full = sms[dev].load();
   if (!full) {
-    cudaError_t e = cudaFuncSetAttribute(kv_move_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(kv_move_kernel<MODE, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(sizeof(MoveSmem)));
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&full, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return launch_error(e);
@@ -466,7 +512,15 @@ int move_pages(const ListArgs& g, long long most, cudaStream_t stream) {
   const long long run = static_cast<long long>(g.c.n_kv) * g.c.page * g.c.hd;
   const long long units = most * g.c.n_layers * 2 * ((run + kMoveChunk - 1) / kMoveChunk);
   const dim3 grid(static_cast<unsigned>(units < full ? units : full));
-  return launch_kernel(kv_move_kernel<MODE>, grid, dim3(kPlanThreads), sizeof(MoveSmem), stream, g);
+  return launch_kernel(kv_move_kernel<MODE, SMALL>, grid, dim3(kPlanThreads), sizeof(MoveSmem), stream, g);
+}
+
+// Every CTA plans for itself where the lists and the tables are small enough.
+template <int MODE>
+int move_pages(const ListArgs& g, long long most, cudaStream_t stream) {
+  const bool small = g.c.n_pages <= 2 * kSmallList && g.n <= kSmallList &&
+                     static_cast<long long>(g.c.max_seqs) * g.c.max_pages <= kSmallTable;
+  return small ? launch_moves<MODE, true>(g, most, stream) : launch_moves<MODE, false>(g, most, stream);
 }
 
 }  // namespace
@@ -477,7 +531,7 @@ using namespace so101;
 
 extern "C" int so101_kv_scratch(const so101_kv_pages* c, int64_t* ints) {
   if (!c || !ints || c->n_pages < 1 || c->max_seqs < 1) return SO101_ERR_ARG;
-  *ints = 4 + 2 * scratch_most(*c) + c->n_pages + c->max_seqs;
+  *ints = 4 + 2 * scratch_most(*c) + c->n_pages + 2LL * c->max_seqs;
   return SO101_OK;
 }
 
@@ -506,7 +560,7 @@ extern "C" int so101_kv_fork(const so101_kv_pages* c, const int* parents, const 
 extern "C" int so101_kv_copy(const so101_kv_pages* c, const int* src, const int* dst, int n, cudaStream_t stream) {
   if (!kv_pages_ok(c) || n < 0 || n > c->n_pages || (n > 0 && (!src || !dst))) return SO101_ERR_ARG;
   if (n == 0) return SO101_OK;
-  return move_pages<kMoveCopy>(list_args(c, src, dst, n), n, stream);
+  return launch_moves<kMoveCopy, false>(list_args(c, src, dst, n), n, stream);
 }
 
 extern "C" int so101_kv_compact(const so101_kv_pages* c, cudaStream_t stream) {

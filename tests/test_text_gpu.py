@@ -512,15 +512,17 @@ class Model:
         self.table = [[to.get(p, p) for p in t] for t in self.table]
 
 
-@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("seed", range(6))
 def test_pages_life(seed):
-    """Random reserves, forks, frees and compactions against the model; what sequences hold stays theirs."""
+    """Random reserves, forks, frees and compactions against the model; what sequences hold stays theirs. The last
+    two have a table and a pool that are too large for a plan in shared memory."""
     from so101_smolvla_edge_b200 import _lib as L
     from so101_smolvla_edge_b200 import ops
     from so101_smolvla_edge_b200.pages import KvPages
 
     rng = random.Random(seed)
-    page, width, pool, n = rng.choice([16, 32, 64]), 6, [40, 3000, 25, 60][seed], [24, 24, 1500, 24][seed]
+    page, width = rng.choice([16, 32, 64]), 6
+    pool, n = [(40, 24), (3000, 24), (25, 1500), (60, 24), (50, 3000), (9000, 24)][seed]
     kv, hd, layers = rng.choice([1, 3]), 64, 2
     c, m = KvPages(layers, pool, kv, hd, n, width * page, page), Model(pool, n, width, page)
     held = {}  # sequence -> its tokens as written (tokens, 2, layers, kv, hd)
