@@ -26,8 +26,8 @@ extern "C" {
  * three (starts: n_seqs + 1 int32, non-decreasing, starts[n_seqs] <= rows; empty sequences are
  * fine); its row r sees its rows 0..r and nothing else, whatever the other rows hold (infinities
  * and NaN included). max_len: at least the longest sequence. cos / sin (rows, hd/2 fp32) rotate q
- * on load (NULL: none); k comes rotated. scale multiplies q.k. hd 64 or 128; 16-byte aligned bases
- * and row strides. Rows outside every sequence are not written. */
+ * on load in fp32 (NULL: none), kept as two bf16 parts at hd 64 and rounded to bf16 at 128; k comes
+ * rotated. scale multiplies q.k. hd 64 or 128; 16-byte aligned bases (cos and sin too) and row strides. Rows outside every sequence are not written. */
 SO101_API int so101_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
                                      int64_t ldv, void* o, int64_t ldo, int64_t rows, const int* starts,
                                      int n_seqs, int64_t max_len, int nq, int nkv, int hd, float scale,
@@ -59,7 +59,8 @@ SO101_API int so101_kv_scratch(const so101_kv_pages* c, int64_t* ints);
  * [starts[i], starts[i+1]) being the LAST tokens of sequence seqs[i] (lengths already count them:
  * so101_kv_reserve; starts NULL: one row per sequence; seqs NULL: sequence i). max_new: at least
  * the most rows of a sequence. cos / sin (rows, hd/2 fp32) rotate the keys first, in fp32, as
- * so101_rope_kv does but without its rounding to bf16 (NULL: none). The rule, per page and head:
+ * so101_rope_kv does but without its rounding to bf16 (NULL: none). k, v, cos, sin 16-byte aligned, ldk and
+ * ldv multiples of 8. The rule, per page and head:
  * scale = 2^e, e = ceil(log2(max |x| / 127)) clamped to [-126, 121]; code = rint(x / scale) clamped
  * to +-127. New tokens in a part-filled page: scale' = max(scale, theirs), older codes become
  * rint(code * scale / scale'). A value that is not finite makes the page's scale NaN for good. */
@@ -77,7 +78,8 @@ SO101_API int so101_kv_read(const so101_kv_pages* c, int layer, const int* start
 /* Attention of each sequence's last tokens over its cached ones. q: (rows, >= nq*hd) bf16, rows
  * [starts[i], starts[i+1]) being the last n_i tokens of sequence seqs[i] (starts NULL: one row
  * per sequence), n_i <= max_q. causal: row r sees tokens <= lengths - n_i + r; otherwise all
- * lengths of them. A row that sees none is 0. o: (rows, nq*hd) bf16. cos / sin rotate q. Probabilities
+ * lengths of them. A row that sees none is 0. o: (rows, nq*hd) bf16. cos / sin rotate q. q, cos and
+ * sin are 16-byte aligned, o 8-byte; ldq is a multiple of 8, ldo of 4. Probabilities
  * are rounded to fp16, sums are fp32. workspace (fp32 partials) and tickets (zero before the first
  * call, left zero) join the parts of a sequence that several CTAs read. */
 SO101_API int so101_attention_pages(const void* q, int64_t ldq, void* o, int64_t ldo, int64_t rows,

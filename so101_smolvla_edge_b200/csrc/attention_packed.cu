@@ -9,17 +9,21 @@
 // sequence's last blocks (most keys) first, in six warp groups that split the registers unevenly:
 //   0  warp 0: TMA, K_j and V_j (128 keys) into rings that run on across items
 //      warps 1, 2: the MMAs of group 0 / 1, S_g = Q_g K_j^T -> TMEM, O_g += P_g V_j, P_g read from TMEM
+//      warp 3: the list of items, ahead of the rest
 //   1  the queries of the next item: loaded, rotated in fp32, rounded to bf16 into swizzled tiles
 //   2-5  the softmax, and O / l to the output rows: two threads per row (TMEM lane)
 // While a group's softmax runs, the tensor pipe works for the other one. TMEM holds S (128 columns), P and O of
 // both groups at head_dim 64; at 128, S and O only, and P takes the place of the S that it came from.
 // Rotated queries are kept in two bf16 parts at head_dim 64 (value and remainder, two MMAs into one S): tensor
-// time is not what bounds it, and the error against 64 bits falls from 2.6e-3 to 2.1e-3 (1.6e-3 is the
+// time is not what bounds it, and the error against 64 bits falls from 2.6e-3 to 1.9e-3 (1.6e-3 is the
 // rounding of the result). At 128 there is no shared memory for the second part: one rounding to bf16.
 // The row maximum is only raised when a tile exceeds it by more than 2^8 (as in the SigLIP kernel).
 // Keys past the row's own token are masked by their index. Their values still meet P = 0 in the MMA, where an
 // infinity or a NaN in a value the row must not see would make the row NaN, so a row whose result is
 // not finite is computed again key by key over what it sees (never with finite values).
+// Measured: one sequence of 8191 tokens, 32 heads on 8 of 128, 620-640 us (0.86-0.89 PFLOP/s; 724 us with a CTA per
+// 128 rows and one softmax thread per row); with heads of 64, 430 us. The chain
+// S -> maximum -> exponentials -> P V -> next S bounds it, with the issue slots half and the tensor pipe 41 to 55% busy.
 #include <atomic>
 #include <cmath>
 
@@ -793,7 +797,7 @@ int launch_packed(const CUtensorMap& tk, const CUtensorMap& tv, PackedArgs a, cu
     sms[dev].store(full);
   }
   // items, at most: the sequences' blocks, one part-filled each, of every kv head. Blocks of 128 rows where all of
-  // them still run at once: a single prompt of 241 tokens takes 11.1 us so, 13.2 with 256.
+  // them still run at once: a single prompt of 241 tokens takes 10.6 us so, 13.0 with 256.
   const int64_t part = a.n_seqs < a.rows ? a.n_seqs : a.rows, stacked = static_cast<int64_t>(a.rows) * a.group;
   const int64_t fine = (stacked / kPkRows + part) * a.n_kv;
   a.block = fine <= full ? kPkRows : 2 * kPkRows;

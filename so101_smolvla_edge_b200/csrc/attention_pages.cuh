@@ -17,6 +17,9 @@
 // 128 sum |q|, far below the 2^-11 that rounding q to f16 does. (In O the same short cut would leave 2^-24 of 128
 // steps beside values that are zero.) Against a prmt under the exponent of 1024 and a subtraction for
 // both, a 32-key tile of 128 dims takes about 250 instructions less of 837.
+// Measured: one sequence of 131071 tokens (32 heads on 8 of 128) 61-64 us, of which about
+// 15 are the start and the join of its parts and the rest runs at the copy rate; 64 ragged sequences, 15 on 5 heads
+// of 64, 46 us, the instructions of the few-row tiles bounding it.
 // Which of a head's dims is which k index of the MMA is free as long as Q and K agree, and so is
 // the order of the keys between S and V, so both are laid out to make a thread's codes contiguous: 16
 // dims of a key row, 8 of a value row, and the pairs of V come from byte permutes of two rows. Q is

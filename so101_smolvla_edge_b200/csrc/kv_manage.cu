@@ -6,7 +6,8 @@
 // same inputs give the same pages, and a call that cannot be met changes nothing. Fork and compact leave
 // a list of page moves, which all CTAs of the same launch carry out. A page is n_layers x 2 runs of
 // n_kv * page * hd bytes (20 KB for five heads of 64 and 64 slots); the runs go through shared
-// memory in bulk copies, eight in flight per SM, bounded by the HBM copy rate.
+// memory in bulk copies, eight in flight per SM, bounded by the HBM copy rate: a compaction that moves 335 MB takes
+// 115 us, 5.8 TB/s read and written (156 us with a launch of its own for the moves and 16-byte loads and stores).
 #include <atomic>
 
 #include "kv_pages.cuh"
@@ -321,7 +322,8 @@ __device__ __forceinline__ void st_release(int* p, int v) {
 // Plan (fork, compact), then move. SMALL: every CTA works the plan out for itself, in shared memory, and starts to
 // copy; the CTA that is last to have done so (an atomic count) then changes the bookkeeping, beside its copies, so
 // that nobody waits. Larger lists and tables: the first CTA to arrive plans for all, in the scratch ints, the
-// others wait (bounded) for its flag. (The flag cost a fork of 64 and a compaction of 20 MB 4 us each.)
+// others wait (bounded) for its flag. (Forks of 64 sequences with part-filled pages of 1.3 MB take
+// 19.5 us, 23.8 with the flag; a compaction that moves 20 MB 15.6 and 17.)
 // Unit u of the moves is (move, layer, keys or values, chunk); CTA b
 // takes units b, b + gridDim.x, ...: all its threads work out the addresses of a batch of them (a single
 // thread that looks each page number up itself moves a unit in 2 us: 266 us for 335 MB), then
