@@ -7,6 +7,8 @@ int attention_pages_64(const PagesArgs& a, int64_t workspace_bytes, int64_t n_ti
   return attention_pages_run<64>(a, workspace_bytes, n_tickets, stream);
 }
 int attention_pages_128(const PagesArgs& a, int64_t workspace_bytes, int64_t n_tickets, cudaStream_t stream);
+// attention_pages_tc.cu
+bool attention_pages_tc(const PagesArgs& a, int64_t workspace_bytes, int64_t n_tickets, cudaStream_t stream, int* rc);
 
 }  // namespace so101
 
@@ -48,9 +50,13 @@ extern "C" int so101_attention_pages(const void* q, int64_t ldq, void* o, int64_
   a.nq = nq;
   a.group = nq / c->n_kv;
   a.causal = causal;
+  a.group_inv = static_cast<uint32_t>(((1ULL << 32) + a.group - 1) / a.group);
+  a.o_wide = a16(o) && ldo % 8 == 0;
   a.n_seqs = n_seqs;
   a.max_q = static_cast<int>(max_q < rows ? max_q : rows);
   a.status = status_ptr();
+  int rc = SO101_OK;
+  if (attention_pages_tc(a, workspace_bytes, n_tickets, stream, &rc)) return rc;
   return c->hd == 64 ? attention_pages_64(a, workspace_bytes, n_tickets, stream)
                      : attention_pages_128(a, workspace_bytes, n_tickets, stream);
 }

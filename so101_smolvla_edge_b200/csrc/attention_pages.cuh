@@ -47,6 +47,8 @@ struct PagesArgs {
   int* tickets;
   float scale_log2;
   int layer, nq, group, causal;
+  uint32_t group_inv;  // 2^32 / group rounded up: x / group is the high word of x * group_inv (x < group + 256)
+  bool o_wide;         // rows of o are 16-byte aligned
   int n_seqs, max_q;
   int* status;
 };
@@ -148,44 +150,63 @@ __device__ __forceinline__ int snap_cut(const PagesPlan& p, int cut, int p0, int
   return min(down, up) > p.slack ? cut : down <= up ? p0 : p0 + steps;
 }
 
-// Steps per (row tile, kv head) and row tiles of entry i.
-template <int HD, int ROWS>
+// Steps of STEP keys per (row tile, kv head) and row tiles of entry i.
+template <int STEP, int ROWS>
 __device__ __forceinline__ void entry_size(const PagesArgs& a, int i, int& steps, int& tiles) {
   const int seq = a.seqs ? __ldg(a.seqs + i) : i;
   const int n = a.starts ? __ldg(a.starts + i + 1) - __ldg(a.starts + i) : 1;
   const int len = seq >= 0 && seq < a.c.max_seqs ? a.c.lengths[seq] : 0;
   const int most = a.c.max_pages * a.c.page;
-  steps = max(1, (min(max(len, 0), most) + PgCfg<HD, ROWS>::kStep - 1) / PgCfg<HD, ROWS>::kStep);
+  steps = max(1, (min(max(len, 0), most) + STEP - 1) / STEP);
   tiles = (min(max(n, 0), a.max_q) * a.group + ROWS - 1) / ROWS;
 }
 
 // Whole CTA: the sum of all entries' steps, then the entry in which the CTA's first step falls. The
 // sums are kept in 32 bits (the host refuses what could pass them).
-template <int HD, int ROWS>
+template <int STEP, int ROWS, int THREADS>
 __device__ __forceinline__ PagesPlan pages_plan(const PagesArgs& a, int* shared) {
+  constexpr int kWarps = THREADS / 32;
+  int* at_cut = shared + 2 * kWarps;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto first_warps = [&](int n) {  // the sum of the first n warps' counts
+    return static_cast<int>(__reduce_add_sync(0xffffffffu, lane < n ? shared[lane] : 0));
+  };
+  int longest = 1;  // most steps of a problem (ROWS > 64)
   auto size = [&](int i) {
     if (i >= a.n_seqs) return 0;
     int steps, tiles;
-    entry_size<HD, ROWS>(a, i, steps, tiles);
+    entry_size<STEP, ROWS>(a, i, steps, tiles);
+    if (tiles > 0) longest = max(longest, steps);
     return steps * tiles * a.c.n_kv;
   };
   const int mine = size(threadIdx.x);  // all entries of a short list
   int sum = mine;
-  for (int i = threadIdx.x + kPgThreads; i < a.n_seqs; i += kPgThreads) sum += size(i);
+  for (int i = threadIdx.x + THREADS; i < a.n_seqs; i += THREADS) sum += size(i);
   sum = __reduce_add_sync(0xffffffffu, sum);
   if (lane == 0) shared[warp] = sum;
+  if (ROWS > 64) {
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0) shared[kWarps + warp] = longest;
+  }
   __syncthreads();
   PagesPlan p;
-  p.total = shared[0] + shared[1] + shared[2] + shared[3];
+  p.total = first_warps(kWarps);
   p.run = max(1, (p.total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
   p.slack = max(p.run / 8, min(2, p.run - 1));
+  if (ROWS > 64) {
+    // Parts of up to 256 rows: written by each and read again by one SM, about half a step's time each, so that the
+    // square root of half the steps is the best run for a problem alone; and a cut costs the time of four steps
+    // (one sequence of 16384 keys, 50 tokens, 32 heads on 8 of 128: 93 us, 108 with runs of total / CTAs).
+    longest = __reduce_max_sync(0xffffffffu, lane < kWarps ? shared[kWarps + lane] : 1);
+    p.run = max(p.run, static_cast<int>(ceilf(sqrtf(0.5f * longest))));
+    p.slack = min(4, p.run / 2);
+  }
   p.entry = p.first = p.begin = p.end = 0;
   const int cut0 = static_cast<int>(blockIdx.x) * p.run, cut1 = cut0 + p.run;
   __syncthreads();
   if (cut0 >= p.total) return p;
   int before = 0;
-  for (int i0 = 0; i0 < a.n_seqs; i0 += kPgThreads) {
+  for (int i0 = 0; i0 < a.n_seqs; i0 += THREADS) {
     const int i = i0 + static_cast<int>(threadIdx.x);
     const int x = i0 ? size(i) : mine;
     int inc = x;
@@ -196,37 +217,43 @@ __device__ __forceinline__ PagesPlan pages_plan(const PagesArgs& a, int* shared)
     }
     if (lane == 31) shared[warp] = inc;
     __syncthreads();
-    int off = before;
-    for (int w = 0; w < warp; ++w) off += shared[w];
-    before += shared[0] + shared[1] + shared[2] + shared[3];
-    const int first = off + inc - x;
+    const int first = before + first_warps(warp) + inc - x;
+    before += first_warps(kWarps);
     if (x > 0) {  // the entries that hold the CTA's two cuts
       if (first <= cut0 && cut0 < first + x) {
         int steps, tiles;
-        entry_size<HD, ROWS>(a, i, steps, tiles);
-        shared[4] = i;
-        shared[5] = first;
-        shared[6] = snap_cut(p, cut0, first + (cut0 - first) / steps * steps, steps);
+        entry_size<STEP, ROWS>(a, i, steps, tiles);
+        at_cut[0] = i;
+        at_cut[1] = first;
+        at_cut[2] = snap_cut(p, cut0, first + (cut0 - first) / steps * steps, steps);
       }
       if (cut1 < p.total && first <= cut1 && cut1 < first + x) {
         int steps, tiles;
-        entry_size<HD, ROWS>(a, i, steps, tiles);
-        shared[7] = snap_cut(p, cut1, first + (cut1 - first) / steps * steps, steps);
+        entry_size<STEP, ROWS>(a, i, steps, tiles);
+        at_cut[3] = snap_cut(p, cut1, first + (cut1 - first) / steps * steps, steps);
       }
     }
     __syncthreads();
     if (cut1 < before) break;
   }
-  p.entry = shared[4];
-  p.first = shared[5];
-  p.begin = shared[6];
-  p.end = cut1 < p.total ? shared[7] : p.total;
+  p.entry = at_cut[0];
+  p.first = at_cut[1];
+  p.begin = at_cut[2];
+  p.end = cut1 < p.total ? at_cut[3] : p.total;
   return p;
 }
 
+// Which CTAs share a problem of `steps` steps from p_first on: cuts b * run inside it, further than the slack from both of
+// its ends, b = low .. high; part 0 is CTA low - 1's, part k CTA low - 1 + k's.
+__device__ __forceinline__ void problem_parts(const PagesPlan& p, int p_first, int steps, int& cta_first, int& parts) {
+  const int low = (p_first + p.slack) / p.run + 1, last = p_first + steps - p.slack - 1;
+  cta_first = low - 1;
+  parts = last > 0 ? max(0, last / p.run - low + 1) + 1 : 1;
+}
+
 // GRAN: slots of a page that a tile holds (a tile is one page, several, or a part of one). Three CTAs per SM (four of the
-// 64-row kernel of head_dim 64) at the price of a few spilled registers: 64 chunks of 50 tokens over 291 keys take
-// 46 us, 57 with two.
+// 64-row kernel of head_dim 64) at the price of a few spilled registers: 64 x 50 tokens of three heads per kv head, in
+// tiles of 64 rows over 291 keys, take 46 us, 57 with two.
 template <int HD, int ROWS, int GRAN>
 __global__ void __launch_bounds__(kPgThreads, HD == 64 && ROWS == 64 ? 4 : 3) attention_pages_kernel(const PagesArgs a) {
   using Cfg = PgCfg<HD, ROWS>;
@@ -254,7 +281,7 @@ __global__ void __launch_bounds__(kPgThreads, HD == 64 && ROWS == 64 ? 4 : 3) at
   }
   grid_dep_launch();
   grid_dep_wait();
-  const PagesPlan plan = pages_plan<HD, ROWS>(a, shared);
+  const PagesPlan plan = pages_plan<Cfg::kStep, ROWS, kPgThreads>(a, shared);
   if (plan.begin >= plan.end) return;
 
   uint8_t* my_ring = smem + ring * Cfg::kRing;
@@ -271,7 +298,7 @@ __global__ void __launch_bounds__(kPgThreads, HD == 64 && ROWS == 64 ? 4 : 3) at
   while (at < plan.end && entry < a.n_seqs) {
     // ---- the problem that step `at` belongs to, and the part of it in this CTA's run
     int steps, tiles_of;
-    entry_size<HD, ROWS>(a, entry, steps, tiles_of);
+    entry_size<Cfg::kStep, ROWS>(a, entry, steps, tiles_of);
     const int entry_end = entry_first + steps * tiles_of * c.n_kv;
     if (at >= entry_end) {
       entry_first = entry_end;
@@ -283,12 +310,8 @@ __global__ void __launch_bounds__(kPgThreads, HD == 64 && ROWS == 64 ? 4 : 3) at
     const int p_first = entry_first + p * steps;
     const int from = at - p_first, to = min(steps, plan.end - p_first);  // its steps here
     at = p_first + to;
-    // cuts b * run inside the problem, further than the slack from both of its ends: b = cut_low ..
-    // cut_high; part 0 is CTA cut_low - 1's, part k CTA cut_low - 1 + k's
-    const int cut_low = (p_first + plan.slack) / plan.run + 1;
-    const int cut_high = (p_first + steps - plan.slack - 1) / plan.run;
-    const int parts = p_first + steps - plan.slack - 1 > 0 ? max(0, cut_high - cut_low + 1) + 1 : 1;
-    const int cta_first = cut_low - 1;
+    int cta_first, parts;
+    problem_parts(plan, p_first, steps, cta_first, parts);
     const int part_no = static_cast<int>(blockIdx.x) - cta_first;
 
     int seq, row0, n_q;
@@ -762,7 +785,8 @@ int dispatch_pages(const PagesArgs& a, int64_t workspace_bytes, int64_t n_ticket
   return launch_pages<HD, ROWS, Cfg::kKeys>(a, most, workspace_bytes, n_tickets, stream);
 }
 
-// rows per CTA: as few as hold a sequence's, up to 64, so that one pass over the keys serves them all
+// rows per CTA: as few as hold a sequence's, up to 64, so that one pass over the keys serves them all (more rows go to
+// the tcgen05 kernel)
 template <int HD>
 int attention_pages_run(const PagesArgs& a, int64_t workspace_bytes, int64_t n_tickets, cudaStream_t stream) {
   const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;

@@ -484,7 +484,7 @@ def pages_workspace(device: int, stream: int) -> Workspace:
     is captured there."""
     ws = _PAGES_WS.get((device, stream))
     if ws is None:
-        ws = _PAGES_WS[device, stream] = Workspace(torch.device("cuda", device), nbytes=32 << 20)
+        ws = _PAGES_WS[device, stream] = Workspace(torch.device("cuda", device), nbytes=40 << 20)
         L.calls().add_workspace(device, stream, ws.partials.data_ptr(), ws.nbytes, ws.tickets.data_ptr(), ws.tickets.numel())
     return ws
 
