@@ -10,7 +10,8 @@
 //   0  warp 0: TMA, K_j and V_j (128 keys) into rings that run on across items
 //      warps 1, 2: the MMAs of group 0 / 1, S_g = Q_g K_j^T -> TMEM, O_g += P_g V_j, P_g read from TMEM
 //      warp 3: the list of items, ahead of the rest
-//   1  the queries of the next item: loaded, rotated in fp32, rounded to bf16 into swizzled tiles
+//   1  the queries of the next item: loaded, rotated in fp32, rounded to bf16 into swizzled tiles (head_dim 128: loaded;
+//      the softmax threads rotate)
 //   2-5  the softmax, and O / l to the output rows: two threads per row (TMEM lane)
 // While a group's softmax runs, the tensor pipe works for the other one. TMEM holds S (128 columns), P and O of
 // both groups at head_dim 64; at 128, S and O only, and P takes the place of the S that it came from.
@@ -73,9 +74,13 @@ struct PkCfg {
   static constexpr uint32_t kColS = 0, kColP = HD == 64 ? 128 : 0, kColO = HD == 64 ? 192 : 128, kGroupCols = 256;
   // Warps: four for loads, MMAs and the item list, then the queries', then 16 for the softmax. Registers per thread
   // of each kind: together no more than the threads start with (80 of 768 threads).
+  // At head_dim 128 the softmax threads turn the queries that those four bring, between an item's last P and its O
+  // (64 prompts of 113 to 305 tokens, 32 heads on 8: 135 us, 182 with the four turning them); at 64, with two buffers, the
+  // four do (15 heads on 5: 54 us, 55; 64 prompts of 512 120 and 129).
+  static constexpr bool kSoftTurns = HD == 128;
   static constexpr int kQWarps = 4;
   static constexpr int kThreads = 32 * (4 + kQWarps + 16);
-  static constexpr int kRegsLoad = HD == 64 ? 40 : 48, kRegsQuery = HD == 64 ? 72 : 48, kRegsSoft = HD == 64 ? 88 : 96;
+  static constexpr int kRegsLoad = HD == 64 ? 40 : 48, kRegsQuery = HD == 64 ? 72 : 40, kRegsSoft = HD == 64 ? 88 : 96;
   static constexpr int kItemReaders = 1 + 4 + kQWarps + 16;  // reads of each item: loads, MMAs 2 x 2 (S, P V), queries, softmax
 };
 static_assert(PkCfg<64>::kSmem <= 232448 && PkCfg<128>::kSmem <= 232448, "227 KB of shared memory per CTA");
@@ -154,16 +159,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // A work item: rows [row_first, row_first + rows) (of the stacked ones) of the sequence that begins at packed
-// row `start`, kv head kvh. rows == 0: no more items.
-struct PackedItem {
+// row `start`, kv head kvh. rows == 0: no more items. What every warp would divide for is worked out with it: row r of the
+// item is token tok + (lead + r) / group, head (lead + r) % group, and row group g has tiles[g] key tiles (0: no rows).
+struct __align__(16) PackedItem {
   int start, row_first, rows, kvh;
+  int tok, lead, tiles[2];
 
-  // Key tiles of row group g (0: none of its rows are there).
-  __device__ __forceinline__ int tiles(const PackedArgs& a, int g, int keys) const {
-    const int here = min(rows - g * kPkRows, kPkRows);
-    return here <= 0 ? 0 : (row_first + g * kPkRows + here - 1) / a.group / keys + 1;
+  __device__ __forceinline__ int tiles_of(int g) const { return g ? tiles[1] : tiles[0]; }
+  __device__ __forceinline__ int all_tiles() const { return max(tiles[0], tiles[1]); }
+  __device__ __forceinline__ void divide(const PackedArgs& a, int keys) {
+    tok = row_first / a.group;
+    lead = row_first - tok * a.group;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int here = min(rows - g * kPkRows, kPkRows);
+      tiles[g] = here <= 0 ? 0 : (tok + ((lead + g * kPkRows + here - 1) * a.group_inv >> 16)) / keys + 1;
+    }
   }
-  __device__ __forceinline__ int tiles(const PackedArgs& a, int keys) const { return max(tiles(a, 0, keys), tiles(a, 1, keys)); }
 };
 
 // The items of one CTA, in order, worked out by one warp for all: item w is kv head w % n_kv of block
@@ -173,7 +185,7 @@ struct PackedItem {
 struct PackedWalk {
   int turn, s0, before;  // items taken; the window's first sequence and the blocks before it
 
-  __device__ __forceinline__ PackedItem next(const PackedArgs& a) {
+  __device__ __forceinline__ PackedItem next(const PackedArgs& a, int keys) {
     const int lane = threadIdx.x & 31;
     const int g = static_cast<int>(gridDim.x), b = static_cast<int>(blockIdx.x);
     const int w = turn * g + (turn & 1 ? g - 1 - b : b);
@@ -181,7 +193,7 @@ struct PackedWalk {
     const int block = w / a.n_kv;
     PackedItem it;
     it.kvh = w - block * a.n_kv;
-    it.start = it.row_first = it.rows = 0;
+    it.start = it.row_first = it.rows = it.tok = it.lead = it.tiles[0] = it.tiles[1] = 0;
     for (; s0 < a.n_seqs; s0 += 32) {
       const int s = s0 + lane;
       int at = 0, len = 0;
@@ -206,6 +218,7 @@ struct PackedWalk {
         const int n = __shfl_sync(0xffffffffu, len, x);
         it.row_first = (before + __shfl_sync(0xffffffffu, inc, x) - 1 - block) * a.block;
         it.rows = min(a.block, n * a.group - it.row_first);
+        it.divide(a, keys);
         return it;
       }
       before += __shfl_sync(0xffffffffu, inc, 31);
@@ -227,8 +240,9 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
   PackedItem* items = reinterpret_cast<PackedItem*>(smem + Cfg::kOffBar);
   uint64_t* item_full = reinterpret_cast<uint64_t*>(items + kPkItems);  // [kPkItems]
   uint64_t* item_empty = item_full + kPkItems;                         // [kPkItems] read by every warp
-  uint64_t* q_full = item_empty + kPkItems;  // [kQBufs] an item's queries are written
-  uint64_t* q_empty = q_full + kQBufs;       // [kQBufs] both groups' S MMAs have read them
+  uint64_t* q_full = item_empty + kPkItems;  // [kQBufs][2] a group's queries of an item are ready
+  uint64_t* q_raw = q_full + 2 * kQBufs;     // [kQBufs] an item's queries are there, to be turned
+  uint64_t* q_empty = q_raw + kQBufs;        // [kQBufs] both groups' S MMAs have read them
   uint64_t* q_first = q_empty + kQBufs;      // [1] the first item's queries are written
   uint64_t* k_full = q_first + 1;            // [kStages]
   uint64_t* k_empty = k_full + kStages;      // [kStages]
@@ -241,7 +255,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
   uint64_t* o_full = p_full + 2;
   uint64_t* o_free = o_full + 2;             // [2] an item's O read out
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
-  static_assert(kPkItems * sizeof(PackedItem) + (2 * kPkItems + 4 + 16 + 4 + 12) * 8 + 4 <= 768, "barrier region");
+  static_assert(kPkItems * sizeof(PackedItem) + (2 * kPkItems + 4 + 4 + 16 + 4 + 12) * 8 + 4 <= 768, "barrier region");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   PackedWalk walk;  // warp 3's
@@ -252,7 +266,9 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       mbar_init(&item_empty[lane], Cfg::kItemReaders);
     }
     if (lane < kQBufs) {
-      mbar_init(&q_full[lane], Cfg::kQWarps);
+      mbar_init(&q_full[2 * lane], a.cos && Cfg::kSoftTurns ? 8 : Cfg::kQWarps);
+      mbar_init(&q_full[2 * lane + 1], a.cos && Cfg::kSoftTurns ? 8 : Cfg::kQWarps);
+      mbar_init(&q_raw[lane], Cfg::kQWarps);
       mbar_init(&q_empty[lane], 2);
     }
     if (lane == 0) mbar_init(q_first, 16);
@@ -273,7 +289,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
   } else if (warp == 3) {  // the first item, beside the set-up
     grid_dep_wait();
     walk.turn = walk.s0 = walk.before = 0;
-    walked = walk.next(a);
+    walked = walk.next(a, kKeys);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -294,11 +310,9 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
   // item i of this CTA; rows == 0 past the last, or where a wait ran out. Each reader takes an item once (a look
   // does not count).
   auto item_at = [&](int i, bool look = false) {
-    PackedItem it;
-    it.start = it.row_first = it.rows = it.kvh = 0;
+    PackedItem it = {};
     if (wait(&item_full[i % kPkItems], i / kPkItems)) {
-      const int4 x = *reinterpret_cast<const int4*>(items + i % kPkItems);
-      it.start = x.x, it.row_first = x.y, it.rows = x.z, it.kvh = x.w;
+      it = items[i % kPkItems];
     }
     __syncwarp();
     if (lane == 0 && !look) mbar_arrive(&item_empty[i % kPkItems]);
@@ -311,10 +325,10 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       // ---- the list of items
       bool ok = true;
       for (int i = 0; ok; ++i) {
-        if (i > 0) walked = walk.next(a);
+        if (i > 0) walked = walk.next(a, kKeys);
         if (i >= kPkItems) ok = wait(&item_empty[i % kPkItems], i / kPkItems - 1);
         if (ok && lane == 0) {
-          *reinterpret_cast<int4*>(items + i % kPkItems) = make_int4(walked.start, walked.row_first, walked.rows, walked.kvh);
+          items[i % kPkItems] = walked;
           mbar_arrive(&item_full[i % kPkItems]);
         }
         __syncwarp();
@@ -332,7 +346,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       for (int i = 0; ok; ++i) {
         const PackedItem it = item_at(i);
         if (it.rows == 0) break;
-        const int n_tiles = it.tiles(a, kKeys);
+        const int n_tiles = it.all_tiles();
         for (int j = 0; j < n_tiles && ok; ++j, ++t) {
           const int st = t % kStages;
           if (t >= kStages) ok = wait(&k_empty[st], t / kStages - 1);
@@ -371,8 +385,8 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
           ++c.item;
           const PackedItem it = item_at(c.item);
           c.j = 0;
-          c.mine = it.tiles(a, g, kKeys);
-          c.tiles = it.rows ? it.tiles(a, kKeys) : 0;
+          c.mine = it.tiles_of(g);
+          c.tiles = it.all_tiles();
         }
         return c.tiles > 0;
       };
@@ -381,7 +395,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
         const int st = cs.t % kStages, qb = cs.item % kQBufs;
         const bool has = cs.j < cs.mine;
         // (q_full[0]'s first use is for item kQBufs)
-        const bool queries = cs.j > 0 || (cs.item == 0 ? wait(q_first, 0) : wait(&q_full[qb], cs.item / kQBufs - (qb == 0 ? 1 : 0)));
+        const bool queries = cs.j > 0 || (cs.item == 0 ? wait(q_first, 0) : wait(&q_full[2 * qb + g], cs.item / kQBufs - (qb == 0 ? 1 : 0)));
         if (!queries || !wait(&k_full[st], cs.t / kStages)) return false;
         // the S before is in registers; where P took its place, P V has read that
         if (has && cs.own > 0 && !(Cfg::kAlias ? pv_done(cs.own - 1) : wait(&s_free[g], cs.own - 1))) return false;
@@ -458,7 +472,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
     }
   } else if (warp < 4 + Cfg::kQWarps) {
     // ---- the queries: 16-byte pieces copied into their swizzled places (all of an item's in flight together),
-    // then, with rotary tables, 8 dims and their partners (HD / 2 later) at a time turned in place
+    // then, with rotary tables and head_dim 64, 8 dims and their partners (HD / 2 later) at a time turned in place
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsQuery));
     constexpr int kPieces = HD / 8, kPairs = HD / 16;
     // the softmax threads bring the first item's queries: at the start they have nothing else to do
@@ -474,7 +488,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       if (!ok) break;
       uint8_t* base = smem + Cfg::kOffQ + 2 * qb * Cfg::kQGroup;
       // row r of the item is token tok0 + (rem0 + r) / group, head (rem0 + r) % group
-      const int tok0 = it.start + it.row_first / a.group, rem0 = it.row_first % a.group;
+      const int tok0 = it.start + it.tok, rem0 = it.lead;
       auto token = [&](int r) { return (rem0 + r) * a.group_inv >> 16; };
       // piece c of row r
       auto at = [&](int r, int c) {
@@ -490,7 +504,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
                      : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      if (a.cos) {
+      if (a.cos && !Cfg::kSoftTurns) {
         // a lane takes 8 dims (and their partners) of a token at a time, for all its heads; the next token's
         // angles are asked for before this one's are used, the first ones beside the copies
         const int first = real > 0 ? token(row0) : 0, tasks = real > 0 ? (token(row0 + real - 1) - first + 1) * kPairs : 0;
@@ -535,7 +549,14 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[qb]);
+      if (lane == 0) {
+        if (a.cos && Cfg::kSoftTurns) {
+          mbar_arrive(&q_raw[qb]);
+        } else {
+          mbar_arrive(&q_full[2 * qb]);
+          mbar_arrive(&q_full[2 * qb + 1]);
+        }
+      }
     }
   } else {
     // ---- softmax of group g: row rl of its 128 (one TMEM lane) by two threads, half hf of every tile's keys
@@ -564,9 +585,9 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       const PackedItem it = item_at(0, true);
       const int r = g * kPkRows + rl;
       if (g * kPkRows < it.rows) {
-        const int row = it.row_first + (r < it.rows ? r : 0), tok = row / a.group;
+        const int row = it.lead + (r < it.rows ? r : 0), t = row * a.group_inv >> 16, tok = it.tok + t;
         const uint4* qr = reinterpret_cast<const uint4*>(a.q + (it.start + tok) * a.ldq +
-                                                         (it.kvh * a.group + row - tok * a.group) * HD);
+                                                         (it.kvh * a.group + row - t * a.group) * HD);
         constexpr int kPairs = HD / 16;
         uint8_t* to = smem + Cfg::kOffQ + g * Cfg::kQGroup + rl * 128;
 #pragma unroll
@@ -601,22 +622,75 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(q_first);
     }
+    // Item i's queries of row rl turned: half of its pairs of pieces, in place (head_dim 128).
+    auto turn = [&](int i) {
+      const PackedItem it = item_at(i, true);
+      if (it.rows == 0) return true;
+      const int qb = i % kQBufs, r = it.lead + g * kPkRows + rl;
+      const bool live = g * kPkRows + rl < it.rows;
+      const long long at = (it.start + it.tok + (live ? r * a.group_inv >> 16 : 0)) * static_cast<long long>(HD / 2);
+      constexpr int kPairs = HD / 16;
+      uint8_t* to = smem + Cfg::kOffQ + (2 * qb + g) * Cfg::kQGroup + rl * 128;
+      bool there = true;
+#pragma unroll
+      for (int c0 = hf * (kPairs / 2); c0 < (hf + 1) * (kPairs / 2); c0 += 2) {
+        float4 ang[2][4];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {  // asked for before the wait
+          const long long x = at + 8 * (c0 + z);
+          ang[z][0] = __ldg(reinterpret_cast<const float4*>(a.cos + x));
+          ang[z][1] = __ldg(reinterpret_cast<const float4*>(a.cos + x + 4));
+          ang[z][2] = __ldg(reinterpret_cast<const float4*>(a.sin + x));
+          ang[z][3] = __ldg(reinterpret_cast<const float4*>(a.sin + x + 4));
+        }
+        if (c0 == hf * (kPairs / 2)) there = wait(&q_raw[qb], i / kQBufs - (qb == 0 ? 1 : 0));
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int c = c0 + z;
+          uint4* u1 = reinterpret_cast<uint4*>(to + c / 8 * Cfg::kQTile + ((c % 8 ^ (rl & 7)) << 4));
+          uint4* u2 = reinterpret_cast<uint4*>(to + (c + kPairs) / 8 * Cfg::kQTile + (((c + kPairs) % 8 ^ (rl & 7)) << 4));
+          uint4 x1 = *u1, x2 = *u2, l1, l2;
+          const float* cv = reinterpret_cast<const float*>(ang[z]);
+          packed_turn<Cfg::kParts>(x1, x2, l1, l2, cv, cv + 8);
+          *u1 = x1;
+          *u2 = x2;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[2 * qb + g]);
+      return there;
+    };
     int t = 0;  // this group's key tiles so far
     bool ok = true;
     for (int item = 0; ok; ++item) {
       const PackedItem it = item_at(item);
       // the two warps of a row meet at every exchange, so they leave together (also after a wait ran out)
       if (fminf(it.rows, other(it.rows)) == 0.f) break;
-      const int n_tiles = it.tiles(a, g, kKeys);
-      if (n_tiles == 0) continue;
+      const int n_tiles = it.tiles_of(g);
+      if (n_tiles == 0) {
+        if (Cfg::kSoftTurns && a.cos && ok) ok = turn(item + 1);
+        continue;
+      }
       const bool live = g * kPkRows + rl < it.rows;
-      const int r = it.row_first + (live ? g * kPkRows + rl : 0);
-      const int tok = r / a.group, head = it.kvh * a.group + r - tok * a.group;
+      const bool idle = g * kPkRows + quad * 32 >= it.rows;  // a warp of padding rows: nobody reads its P
+      const int r = it.lead + (live ? g * kPkRows + rl : 0), past = r * a.group_inv >> 16;
+      const int tok = it.tok + past, head = it.kvh * a.group + r - past * a.group;
       const int vis = (live ? tok + 1 : 1) - hf * kMine;  // of its half's keys, [0, vis) are visible to this row
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n_tiles; ++j, ++t) {
         if (ok) ok = wait(&s_full[g], t);
         tc_fence_after();
+        if (idle) {
+          if (j > 0 && ok) ok = pv_done(t - 1);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (!Cfg::kAlias) mbar_arrive(&s_free[g]);
+            mbar_arrive(&p_full[g]);
+          }
+          continue;
+        }
         uint32_t sv[kMine];
 #pragma unroll
         for (int c = 0; c < kMine; c += 32) tmem_ld32(s_addr + c, sv + c);
@@ -627,10 +701,15 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
           if (lane == 0) mbar_arrive(&s_free[g]);
         }
         const int nvis = vis - j * kKeys;
-        if (nvis < kMine) {
+        if (nvis < kMine) {  // by bits: several become predicates in one instruction
 #pragma unroll
-          for (int e = 0; e < kMine; ++e)
-            if (e >= nvis) sv[e] = __float_as_uint(-INFINITY);
+          for (int c = 0; c < kMine; c += 32) {
+            const int n = nvis - c;
+            const uint32_t seen = n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen & 1u << e)) sv[c + e] = __float_as_uint(-INFINITY);
+          }
         }
         auto tile_max = [&]() {
           float mx[4];  // three operands at a time
@@ -688,6 +767,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[g]);
       }
+      if (Cfg::kSoftTurns && a.cos && ok) ok = turn(item + 1);  // while the last P V runs
       l += other(l);
       if (ok) ok = pv_done(t - 1);
       tc_fence_after();

@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
           do {
             const PtItem it = item_at(++x.item);
             if (it.rows == 0) return false;
-            x.mine = it.tiles[g];
+            x.mine = g ? it.tiles[1] : it.tiles[0];
             x.tiles = tiles_all(it);
           } while (x.tiles == 0);
         }
@@ -798,8 +798,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
           const bool edge = __any_sync(0xffffffffu, nvis < kMine);
           if (edge) {
 #pragma unroll
-            for (int e = 0; e < kMine; ++e)
-              if (e >= nvis) sv[e] = __float_as_uint(-INFINITY);
+            for (int c = 0; c < kMine; c += 32) {
+              const int n = nvis - c;
+              const uint32_t seen = n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u;
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(seen & 1u << e)) sv[c + e] = __float_as_uint(-INFINITY);
+            }
           }
           float m_tile = -INFINITY, mul[kMine / 16];
 #pragma unroll
