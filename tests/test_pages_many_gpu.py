@@ -149,3 +149,15 @@ def test_rows_at_eight_bytes_and_graph():
     g.replay()
     check(out, *pages_want(q, c, 0, 6, counts, range(2), True, 0.125))
     assert (wide[:, :4] == 0).all()
+
+
+@pytest.mark.parametrize("rows,heads", [(66, 1), (1, 3), (13, 2)])
+def test_long_lists(rows, heads):
+    """More sequences than a CTA's threads look at in one pass, some empty, one long among them."""
+    lens = [(37 * i) % 90 for i in range(1000)]
+    lens[700] = 3000
+    counts = [rows if i % 7 else 0 for i in range(1000)] if rows > 1 else [1] * 1000
+    c = cache(lens, 1, 64, 16, seed=121)
+    q = queries(sum(counts), heads, 64, seed=122)
+    got = run(c, q, heads, counts, range(1000))
+    check(got, *pages_want(q, c, 0, heads, counts, range(1000), True, 0.125))
