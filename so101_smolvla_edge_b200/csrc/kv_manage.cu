@@ -7,8 +7,9 @@
 // a list of page moves, which all CTAs of the same launch carry out. A page is n_layers x 2 runs of
 // n_kv * page * hd bytes (20 KB for five heads of 64 and 64 slots); the runs go through shared
 // memory in bulk copies, eight in flight per SM, bounded by the HBM copy rate: a compaction that moves 335 MB takes
-// 115 us, 5.8 TB/s read and written (156 us with a launch of its own for the moves and 16-byte loads and stores).
+// 113 us, 5.9 TB/s read and written (156 us with a launch of its own for the moves and 16-byte loads and stores).
 #include <atomic>
+#include <type_traits>
 
 #include "kv_pages.cuh"
 
@@ -59,28 +60,24 @@ __device__ __forceinline__ int block_scan(int x, int& total, int* warp_sums) {
   }
   if (lane == 31) warp_sums[warp] = inc;
   __syncthreads();
-  if (warp == 0) {
-    int w = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, d);
-      if (lane >= d) w += y;
-    }
-    warp_sums[lane] = w;
-  }
-  __syncthreads();
-  const int before = warp ? warp_sums[warp - 1] : 0;
-  total = warp_sums[kPlanThreads / 32 - 1];
+  const int w = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
+  const int before = static_cast<int>(__reduce_add_sync(0xffffffffu, lane < warp ? w : 0));
+  total = static_cast<int>(__reduce_add_sync(0xffffffffu, w));
   __syncthreads();
   return before + inc - x;
 }
 
-// The lowest `want` free pages, ascending, into list; false if there are fewer. Whole CTA.
-__device__ __forceinline__ bool free_pages(const KvPages& c, int want, int* list, int* warp_sums) {
+// The count of the thread's page among the first kPlanThreads; asked for early, beside other look-ups.
+__device__ __forceinline__ int first_ref(const KvPages& c) {
+  return static_cast<int>(threadIdx.x) < c.n_pages ? c.refs[threadIdx.x] : 1;
+}
+
+// The lowest `want` free pages, ascending, into list; false if there are fewer. Whole CTA; first: first_ref.
+__device__ __forceinline__ bool free_pages(const KvPages& c, int want, int* list, int* warp_sums, int first) {
   int found = 0;
   for (int p0 = 0; p0 < c.n_pages && found < want; p0 += kPlanThreads) {
     const int p = p0 + static_cast<int>(threadIdx.x);
-    const int free = p < c.n_pages && c.refs[p] <= 0 ? 1 : 0;
+    const int free = p < c.n_pages && (p0 ? c.refs[p] : first) <= 0 ? 1 : 0;
     int here;
     const int rank = found + block_scan(free, here, warp_sums);
     if (free && rank < want) list[rank] = p;
@@ -110,6 +107,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_reserve_kernel(const ListA
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
   // pages that each entry needs, as running offsets
+  const int first = first_ref(c);
   int want = 0;
   for (int i0 = 0; i0 < g.n; i0 += kPlanThreads) {
     const int i = i0 + static_cast<int>(threadIdx.x);
@@ -129,7 +127,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_reserve_kernel(const ListA
     if (here > c.n_pages) bad = 1;
   }
   __syncthreads();
-  const bool enough = !bad && want <= c.n_pages && free_pages(c, want, s.src, warp_sums);
+  const bool enough = !bad && want <= c.n_pages && free_pages(c, want, s.src, warp_sums, first);
   if (!enough) {
     if (threadIdx.x == 0) record_error(g.status, SO101_ERR_PAGES);
     return;
@@ -194,6 +192,7 @@ __device__ __forceinline__ int plan_fork(const ListArgs& g, const MovePlan& m, i
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
   int copies = 0;
+  const int first = first_ref(c);
   for (int i0 = 0; i0 < g.n; i0 += kPlanThreads) {
     const int i = i0 + static_cast<int>(threadIdx.x);
     int part = 0, len = 0;
@@ -207,14 +206,15 @@ __device__ __forceinline__ int plan_fork(const ListArgs& g, const MovePlan& m, i
       part = len % c.page ? 1 : 0;
       m.len[i] = len;
     }
+    const int page = part ? c.table[static_cast<long long>(g.a[i]) * c.max_pages + len / c.page] : 0;
     int here;
     const int off = copies + block_scan(part, here, warp_sums);
     if (i < g.n) m.place[i] = part ? off : -1;
-    if (part) m.src[off] = c.table[static_cast<long long>(g.a[i]) * c.max_pages + len / c.page];
+    if (part) m.src[off] = page;
     copies += here;
   }
   __syncthreads();
-  return !bad && copies <= c.n_pages && free_pages(c, copies, m.dst, warp_sums) ? copies : -1;
+  return !bad && copies <= c.n_pages && free_pages(c, copies, m.dst, warp_sums, first) ? copies : -1;
 }
 
 // The bookkeeping of a planned fork, a warp per entry, by warps [first, first + warps) of the CTA.
@@ -246,13 +246,21 @@ __device__ __forceinline__ void apply_fork(const ListArgs& g, const MovePlan& m,
 __device__ __forceinline__ int plan_compact(const ListArgs& g, const MovePlan& m, int* warp_sums) {
   const KvPages& c = g.c;
   int live = 0;
-  for (int p = threadIdx.x; p < c.n_pages; p += kPlanThreads) live += c.refs[p] > 0 ? 1 : 0;
+  uint32_t seen = 0u;  // of the thread's first 32 pages, which are in use
+#pragma unroll 4
+  for (int i = 0; i * kPlanThreads < c.n_pages; ++i) {
+    const int p = i * kPlanThreads + static_cast<int>(threadIdx.x);
+    if (p < c.n_pages && c.refs[p] > 0) {
+      ++live;
+      if (i < 32) seen |= 1u << i;
+    }
+  }
   int total;
   block_scan(live, total, warp_sums);
   int high = 0, holes = 0;
-  for (int p0 = 0; p0 < c.n_pages; p0 += kPlanThreads) {
+  for (int p0 = 0, i = 0; p0 < c.n_pages; p0 += kPlanThreads, ++i) {
     const int p = p0 + static_cast<int>(threadIdx.x);
-    const bool used = p < c.n_pages && c.refs[p] > 0;
+    const bool used = i < 32 ? seen >> i & 1u : p < c.n_pages && c.refs[p] > 0;
     const int move = used && p >= total, hole = p < c.n_pages && !used && p < total;
     int sum;  // both counts in one scan: at most 512 of each per turn
     const int off = block_scan(move | hole << 16, sum, warp_sums);
@@ -322,8 +330,9 @@ __device__ __forceinline__ void st_release(int* p, int v) {
 // Plan (fork, compact), then move. SMALL: every CTA works the plan out for itself, in shared memory, and starts to
 // copy; the CTA that is last to have done so (an atomic count) then changes the bookkeeping, beside its copies, so
 // that nobody waits. Larger lists and tables: the first CTA to arrive plans for all, in the scratch ints, the
-// others wait (bounded) for its flag. (Forks of 64 sequences with part-filled pages of 1.3 MB take
-// 19.5 us, 23.8 with the flag; a compaction that moves 20 MB 15.6 and 17.)
+// others wait (bounded) for its flag. (64 sequences freed and forked again, their part-filled pages 1.3 MB each:
+// 17.5 us, 23.8 with the flag. The count is asked for by the threads that do not copy: 19.5 with the copies behind it
+// and each look-up behind the one before.)
 // Unit u of the moves is (move, layer, keys or values, chunk); CTA b
 // takes units b, b + gridDim.x, ...: all its threads work out the addresses of a batch of them (a single
 // thread that looks each page number up itself moves a unit in 2 us: 266 us for 335 MB), then
@@ -345,22 +354,22 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs
   int moves = g.n;
   bool settle = false;   // this CTA changes the bookkeeping
   bool planned = true;
+  // whether the CTA, having planned, is the last to have done so (one thread of each asks)
+  auto planned_last = [&]() {
+    __threadfence();
+    const bool last = atomicAdd(s.left, 1) == static_cast<int>(gridDim.x) - 1;
+    if (last) *s.left = 0;
+    __threadfence();
+    return last;
+  };
   MovePlan m = {s.src, s.dst, s.aux, s.place};
   if (SMALL) m = {sm.src, sm.dst, sm.len, sm.place};
   if (MODE != kMoveCopy && SMALL) {
     __syncthreads();
     moves = MODE == kMoveFork ? plan_fork(g, m, warp_sums) : plan_compact(g, m, warp_sums);
     __syncthreads();
-    if (threadIdx.x == 0) {
-      __threadfence();
-      shared = atomicAdd(s.left, 1) == static_cast<int>(gridDim.x) - 1;
-      if (shared) *s.left = 0;
-      __threadfence();
-    }
-    __syncthreads();
-    settle = shared;
     if (moves < 0) {
-      if (settle && threadIdx.x == 0) record_error(g.status, SO101_ERR_PAGES);
+      if (threadIdx.x == 0 && planned_last()) record_error(g.status, SO101_ERR_PAGES);
       return;
     }
   } else if (MODE != kMoveCopy) {
@@ -400,21 +409,26 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs
   const int run = c.n_kv * c.page * c.hd;  // bytes per move, layer, keys or values
   const int chunks = (run + kMoveChunk - 1) / kMoveChunk;
   const int chunk = ((run + chunks - 1) / chunks + 15) / 16 * 16;
-  const long long units = static_cast<long long>(moves) * c.n_layers * 2 * chunks;
+  using Count = typename std::conditional<SMALL, unsigned, long long>::type;  // (the host sees to their size)
+  const Count units = static_cast<Count>(moves) * c.n_layers * 2 * chunks;
   // the scales, and after a compaction the tables: by the warps that do not copy
   auto small_work = [&]() {
     const int t = static_cast<int>(threadIdx.x) - 32, step = kPlanThreads - 32;
-    const long long scales = static_cast<long long>(moves) * c.n_layers * c.n_kv * 2;
-    for (long long e = static_cast<long long>(blockIdx.x) * step + t; e < scales;
-         e += static_cast<long long>(gridDim.x) * step) {
+    const Count scales = static_cast<Count>(moves) * c.n_layers * c.n_kv * 2;
+    for (Count e = static_cast<Count>(blockIdx.x) * step + t; e < scales; e += static_cast<Count>(gridDim.x) * step) {
       const int which = static_cast<int>(e & 1);
       const int h = static_cast<int>((e >> 1) % c.n_kv);
-      const long long w = (e >> 1) / c.n_kv;
+      const Count w = (e >> 1) / c.n_kv;
       const int layer = static_cast<int>(w % c.n_layers), k = static_cast<int>(w / c.n_layers);
       const int from = src_of(k), to = dst_of(k);
       if (from < 0 || from >= c.n_pages || to < 0 || to >= c.n_pages) continue;
       float* sc = which ? c.v_scale : c.k_scale;
       sc[kv_scale_at(c, layer, to, h)] = sc[kv_scale_at(c, layer, from, h)];
+    }
+    if (MODE != kMoveCopy && SMALL) {
+      if (t == 0) shared = planned_last();
+      asm volatile("bar.sync 1, %0;" ::"r"(step) : "memory");
+      settle = shared;
     }
     if (MODE == kMoveFork && SMALL && settle) apply_fork(g, m, 1, kPlanThreads / 32 - 1);
     if (MODE == kMoveCompact && (SMALL ? settle : planned)) {
@@ -427,14 +441,14 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_move_kernel(const ListArgs
       }
     }
   };
-  const long long mine = units > blockIdx.x ? (units - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+  const Count mine = units > blockIdx.x ? (units - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
   constexpr int kAhead = kMoveStages / 2;
   bool ok = true;
-  for (long long i0 = 0; i0 < mine || i0 == 0; i0 += kMoveBatch) {
-    const int n = static_cast<int>(max(0LL, min(static_cast<long long>(kMoveBatch), mine - i0)));
+  for (Count i0 = 0; i0 < mine || i0 == 0; i0 += kMoveBatch) {
+    const int n = static_cast<int>(mine - i0 < kMoveBatch ? mine - i0 : kMoveBatch);
     __syncthreads();  // thread 0 is done with the batch before
     for (int i = threadIdx.x; i < n; i += kPlanThreads) {
-      const long long u = blockIdx.x + (i0 + i) * gridDim.x, w = u / chunks;
+      const Count u = blockIdx.x + (i0 + i) * gridDim.x, w = u / chunks;
       const int off = static_cast<int>(u % chunks) * chunk;
       const int layer = static_cast<int>((w >> 1) % c.n_layers), k = static_cast<int>((w >> 1) / c.n_layers);
       const int from = src_of(k), to = dst_of(k);
@@ -520,8 +534,11 @@ int launch_moves(const ListArgs& g, long long most, cudaStream_t stream) {
 // Every CTA plans for itself where the lists and the tables are small enough.
 template <int MODE>
 int move_pages(const ListArgs& g, long long most, cudaStream_t stream) {
+  const long long run = static_cast<long long>(g.c.n_kv) * g.c.page * g.c.hd;
+  const long long units = 2LL * kSmallList * g.c.n_layers * ((run + kMoveChunk - 1) / kMoveChunk);  // at most
   const bool small = g.c.n_pages <= 2 * kSmallList && g.n <= kSmallList &&
-                     static_cast<long long>(g.c.max_seqs) * g.c.max_pages <= kSmallTable;
+                     static_cast<long long>(g.c.max_seqs) * g.c.max_pages <= kSmallTable && units < (1LL << 30) &&
+                     2LL * kSmallList * g.c.n_layers * g.c.n_kv < (1LL << 30);
   return small ? launch_moves<MODE, true>(g, most, stream) : launch_moves<MODE, false>(g, most, stream);
 }
 
