@@ -19,7 +19,7 @@
 // both, a 32-key tile of 128 dims takes about 250 instructions less of 837.
 // Measured: one sequence of 131071 tokens (32 heads on 8 of 128) 61-64 us, of which about
 // 15 are the start and the join of its parts and the rest runs at the copy rate; 64 ragged sequences, 15 on 5 heads
-// of 64, 46 us, the instructions of the few-row tiles bounding it.
+// of 64, 46 us, bounded by the latency of the few-row tiles with three warps per scheduler.
 // Which of a head's dims is which k index of the MMA is free as long as Q and K agree, and so is
 // the order of the keys between S and V, so both are laid out to make a thread's codes contiguous: 16
 // dims of a key row, 8 of a value row, and the pairs of V come from byte permutes of two rows. Q is
