@@ -60,7 +60,7 @@ struct PtCfg {
   static constexpr uint32_t kColS = 0, kColP = HD == 64 ? 128 : 0, kColO = HD == 64 ? 192 : 128, kGroupCols = 256;
   static constexpr int kRegsLoad = 40, kRegsQuery = 64, kRegsOps = 48, kRegsSoft = 88;
   // together 64512: the 72 each that the threads start with
-  static constexpr int kItemReaders = 1 + 4 + 4 + 4 + 16;
+  static constexpr int kItemReaders = 1 + 2 + 4 + 4 + 16;  // reads of each item: codes, MMAs, queries, operands, softmax
 };
 static_assert(kPtSlots >= PtCfg<64>::kRaws + PtCfg<64>::kStages && kPtSlots >= PtCfg<128>::kRaws + PtCfg<128>::kStages,
               "a tile's scales are written while operands up to kRaws + kStages - 1 tiles back may be in use");
@@ -484,29 +484,30 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
       constexpr uint32_t ID_S = idesc_attn(kPtKeys, 0) & kF16;
       constexpr uint32_t ID_O = idesc_attn(64, 1) & kF16;
       const uint32_t d0 = tmem + g * Cfg::kGroupCols;
+      // Both cursors are in one item: the next is looked for when the last P V of this one is issued.
       struct Cursor {
-        int item, j, t, mine, tiles, own, with;  // with: items that had tiles, before this
-      } cs = {-1, 0, -1, 0, 0, 0, -1}, cp = {-1, 0, -1, 0, 0, 0, -1};
+        int j, t, own;  // tile of the item, of the CTA; own tiles so far
+      } cs = {0, -1, 0}, cp = {0, -1, 0};
+      int item = -1, with = -1, mine = 0, tiles = 0;  // with: items that had tiles, before this; this group's tiles, all
       int n_items = 0;
       auto pv_done = [&](int n) { return wait(&o_full[g], n); };
-      auto step = [&](Cursor& x) {
-        ++x.t;
-        if (x.item < 0 || ++x.j == x.tiles) {
-          x.j = 0;
-          ++x.with;
-          do {
-            const PtItem it = item_at(++x.item);
-            if (it.rows == 0) return false;
-            x.mine = g ? it.tiles[1] : it.tiles[0];
-            x.tiles = tiles_all(it);
-          } while (x.tiles == 0);
-        }
+      // To the next item that has tiles; false past the last. The list's slots go round only as the softmax ends items,
+      // and a row of items without tiles can be longer than the list: so each is read once, with no P V outstanding.
+      auto seek = [&]() {
+        do {
+          const PtItem it = item_at(++item);
+          if (it.rows == 0) return false;
+          mine = g ? it.tiles[1] : it.tiles[0];
+          tiles = tiles_all(it);
+        } while (tiles == 0);
+        cs.j = cp.j = 0;
+        ++with;
         return true;
       };
       auto issue_s = [&]() {
-        const int st = cs.t % kStages, qb = cs.with % kQBufs;
-        const bool has = cs.j < cs.mine;
-        if (!((cs.j > 0 || wait(&q_full[qb], cs.with / kQBufs)) && wait(&k_full[st], cs.t / kStages))) return false;
+        const int st = ++cs.t % kStages, qb = with % kQBufs;
+        const bool has = cs.j < mine;
+        if (!((cs.j > 0 || wait(&q_full[qb], with / kQBufs)) && wait(&k_full[st], cs.t / kStages))) return false;
         if (has && cs.own > 0 && !(Cfg::kAlias ? pv_done(cs.own - 1) : wait(&s_free[g], cs.own - 1))) return false;
         tc_fence_after();
         if (elect_one()) {
@@ -523,17 +524,18 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
           } else {
             mbar_arrive(&k_empty[st]);
           }
-          if (cs.j + 1 == cs.tiles) {
-            if (cs.mine > 0) mma_commit(&q_empty[qb]);
+          if (cs.j + 1 == tiles) {
+            if (mine > 0) mma_commit(&q_empty[qb]);
             else mbar_arrive(&q_empty[qb]);
           }
         }
         if (has) ++cs.own;
+        ++cs.j;
         return true;
       };
       auto issue_pv = [&]() {
-        const int st = cp.t % kStages;
-        const bool has = cp.j < cp.mine;
+        const int st = ++cp.t % kStages;
+        const bool has = cp.j < mine;
         if (!wait(&v_full[st], cp.t / kStages) || (has && !wait(&p_full[g], cp.own))) return false;
         if (has && cp.j == 0 && n_items > 0 && !wait(&o_free[g], n_items - 1)) return false;
         tc_fence_after();
@@ -557,20 +559,19 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
           ++cp.own;
           if (cp.j == 0) ++n_items;
         }
+        ++cp.j;
         return true;
       };
       // S runs a tile ahead of P V; after it, an item's first S (whose queries may not be there yet) and S in the
       // place of P
-      int ahead = 0;
-      bool ok = true, s_more = step(cs);
-      while (ok && (s_more || ahead > 0)) {
-        if (s_more && (ahead == 0 || (ahead == 1 && !Cfg::kAlias && cs.j > 0))) {
-          ok = issue_s();
-          if (ok) s_more = step(cs);
-          ++ahead;
-        } else {
-          ok = step(cp) && issue_pv();
-          --ahead;
+      bool ok = true;
+      while (ok && seek()) {
+        while (ok && cp.j < tiles) {
+          const int ahead = cs.j - cp.j;
+          if (cs.j < tiles && (ahead == 0 || (ahead == 1 && !Cfg::kAlias)))
+            ok = issue_s();
+          else
+            ok = issue_pv();
         }
       }
     }
