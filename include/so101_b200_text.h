@@ -39,7 +39,7 @@ SO101_API int so101_attention_packed(const void* q, int64_t ldq, const void* k, 
  * value being code * scale. refs[p] counts the sequences that hold page p (0: free). table rows
  * hold -1 past a sequence's pages. page 16, 32 or 64; hd 64 or 128; k, v, k_scale, v_scale
  * 16-byte aligned. scratch: so101_kv_scratch ints, zero before the first call, used by
- * reserve, fork and compact, which must be ordered on one stream. */
+ * reserve, free, append, fork and compact, which must be ordered on one stream. */
 typedef struct so101_kv_pages {
   int8_t* k;
   int8_t* v;
@@ -63,7 +63,9 @@ SO101_API int so101_kv_scratch(const so101_kv_pages* c, int64_t* ints);
  * ldv multiples of 8. The rule, per page and head:
  * scale = 2^e, e = ceil(log2(max |x| / 127)) clamped to [-126, 121]; code = rint(x / scale) clamped
  * to +-127. New tokens in a part-filled page: scale' = max(scale, theirs), older codes become
- * rint(code * scale / scale'). A value that is not finite makes the page's scale NaN for good. */
+ * rint(code * scale / scale'). A value that is not finite makes the page's scale NaN for good.
+ * A sequence whose last so101_kv_reserve was refused takes no rows (its length does not count them:
+ * they would replace older tokens) until one is met or it is freed; SO101_ERR_PAGES is recorded. */
 SO101_API int so101_kv_append(const so101_kv_pages* c, int layer, const void* k, int64_t ldk, const void* v,
                               int64_t ldv, int64_t rows, const int* starts, const int* seqs, int n_seqs,
                               int64_t max_new, const float* cos, const float* sin, cudaStream_t stream);
@@ -91,7 +93,8 @@ SO101_API int so101_attention_pages(const void* q, int64_t ldq, void* o, int64_t
                                     cudaStream_t stream);
 
 /* lengths[seqs[i]] += tokens[i], taking the lowest free pages in the order of the list. If any
- * sequence would pass max_pages * page tokens or the pages do not suffice, nothing changes and
+ * sequence would pass max_pages * page tokens or the pages do not suffice, nothing changes,
+ * so101_kv_append takes no rows of these sequences until a call for them is met, and
  * SO101_ERR_PAGES is recorded. The sequences of a call are distinct. */
 SO101_API int so101_kv_reserve(const so101_kv_pages* c, const int* seqs, const int* tokens, int n,
                                cudaStream_t stream);

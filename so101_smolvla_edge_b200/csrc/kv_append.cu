@@ -19,6 +19,7 @@ struct AppendArgs {
   long long rows;
   const int* starts;
   const int* seqs;
+  const int* refused;
   const float* cos;
   const float* sin;
   int layer;
@@ -70,9 +71,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendA
   const int head = blockIdx.y >> 1, which = blockIdx.y & 1;
   int seq, row0, n;
   if (!kv_rows(c, a.starts, a.seqs, blockIdx.z, a.rows, seq, row0, n, a.status)) return;
+  const int refused = a.refused[seq];  // there is no room for these rows: the length does not count them
   const int len = kv_length(c, seq, a.status);
   const int old = len - n;
-  if (old < 0) {
+  if (old < 0 || (refused && n > 0)) {
     if (threadIdx.x == 0) record_error(a.status, SO101_ERR_PAGES);
     return;
   }
@@ -276,6 +278,7 @@ extern "C" int so101_kv_append(const so101_kv_pages* c, int layer, const void* k
   a.rows = rows;
   a.starts = starts;
   a.seqs = seqs;
+  a.refused = c->scratch + kv_refused_at(*c);
   a.cos = cos;
   a.sin = sin;
   a.layer = layer;

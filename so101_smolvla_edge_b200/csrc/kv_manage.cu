@@ -17,10 +17,8 @@ namespace so101 {
 
 constexpr int kPlanThreads = 512;
 
-// Scratch ints: number of moves, arrivals, the plan's flag and departures (the last three zero between
-// calls), then src[most], dst[most] (most = max(n_pages, max_seqs)), then
-// remap[n_pages], and per list entry running offsets or parents' lengths [max_seqs] and places [max_seqs].
-struct Scratch {
+struct Scratch {  // kv_pages.cuh: kv_refused_at
+
   int* moves;
   int* arrived;
   int* ready;
@@ -30,12 +28,11 @@ struct Scratch {
   int* remap;
   int* aux;
   int* place;
+  int* refused;
 };
 
-__host__ __device__ inline long long scratch_most(const KvPages& c) { return c.n_pages > c.max_seqs ? c.n_pages : c.max_seqs; }
-
 __device__ __forceinline__ Scratch scratch_of(const KvPages& c) {
-  const long long most = scratch_most(c);
+  const long long most = kv_scratch_most(c);
   Scratch s;
   s.moves = c.scratch;
   s.arrived = c.scratch + 1;
@@ -46,6 +43,7 @@ __device__ __forceinline__ Scratch scratch_of(const KvPages& c) {
   s.remap = s.dst + most;
   s.aux = s.remap + c.n_pages;
   s.place = s.aux + c.max_seqs;
+  s.refused = c.scratch + kv_refused_at(c);
   return s;
 }
 
@@ -130,6 +128,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_reserve_kernel(const ListA
   const bool enough = !bad && want <= c.n_pages && free_pages(c, want, s.src, warp_sums, first);
   if (!enough) {
     if (threadIdx.x == 0) record_error(g.status, SO101_ERR_PAGES);
+    // the lengths stay, so what is appended next would land on older tokens: kv_append leaves these sequences alone
+    for (int i = threadIdx.x; i < g.n; i += kPlanThreads)
+      if (g.a[i] >= 0 && g.a[i] < c.max_seqs) s.refused[g.a[i]] = 1;
     return;
   }
   for (int i = threadIdx.x >> 5; i < g.n; i += kPlanThreads / 32) {  // a warp per entry
@@ -142,7 +143,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_reserve_kernel(const ListA
       c.refs[id] = 1;
     }
     __syncwarp();
-    if (lane == 0) c.lengths[seq] = len + add;
+    if (lane == 0) {
+      c.lengths[seq] = len + add;
+      s.refused[seq] = 0;
+    }
   }
 }
 
@@ -161,6 +165,7 @@ __global__ void __launch_bounds__(kFreeThreads) kv_free_kernel(const ListArgs g)
     return;
   }
   int len = lane == 0 ? atomicExch(c.lengths + seq, 0) : 0;
+  if (lane == 0) c.scratch[kv_refused_at(c) + seq] = 0;
   len = __shfl_sync(0xffffffffu, len, 0);
   int* row = c.table + static_cast<long long>(seq) * c.max_pages;
   const int held = min(pages_for(c, max(len, 0)), c.max_pages);
@@ -550,7 +555,7 @@ using namespace so101;
 
 extern "C" int so101_kv_scratch(const so101_kv_pages* c, int64_t* ints) {
   if (!c || !ints || c->n_pages < 1 || c->max_seqs < 1) return SO101_ERR_ARG;
-  *ints = 4 + 2 * scratch_most(*c) + c->n_pages + 2LL * c->max_seqs;
+  *ints = kv_refused_at(*c) + c->max_seqs;
   return SO101_OK;
 }
 

@@ -20,6 +20,15 @@ inline bool kv_pages_ok(const KvPages* c) {
   return c->hd == 64 || c->hd == 128;
 }
 
+// The scratch ints: number of moves, arrivals, the plan's flag and departures (the last three zero between
+// calls), then src[most], dst[most] (most = max(n_pages, max_seqs)), then remap[n_pages], per list entry running
+// offsets or parents' lengths [max_seqs] and places [max_seqs], and per sequence whether its last reservation was
+// refused [max_seqs].
+__host__ __device__ inline long long kv_scratch_most(const KvPages& c) { return c.n_pages > c.max_seqs ? c.n_pages : c.max_seqs; }
+__host__ __device__ inline long long kv_refused_at(const KvPages& c) {
+  return 4 + 2 * kv_scratch_most(c) + c.n_pages + 2LL * c.max_seqs;
+}
+
 // Element offset of (layer, page id, kv head) in the code arrays (slot 0, dim 0) and in the scales.
 // A long cache passes 32 bits.
 __device__ __forceinline__ long long kv_scale_at(const KvPages& c, int layer, int id, int head) {

@@ -535,6 +535,7 @@ def kv_append(
     tokens of sequence seqs[i], which `kv_reserve` has already counted into its length; at most
     max_new per sequence. starts=None: one row per sequence; seqs=None: sequence i. cos and sin (rows,
     hd / 2) rotate the keys in fp32 before they are quantised. Appending the same rows again changes nothing.
+    A sequence whose last `kv_reserve` was refused takes no rows (they would replace older tokens); ERR_PAGES is recorded.
     """
     L.calls().kv_append(pages.handle, layer, k, v, starts, seqs, max_new, cos, sin)
 
@@ -581,7 +582,8 @@ def attention_pages(
 def kv_reserve(pages: KvPages, seqs: torch.Tensor, tokens: torch.Tensor) -> None:
     """Sequence seqs[i] grows by tokens[i] (int32, on the device): its length now, its pages from the
     lowest free ones. The sequences are distinct. A call that cannot be met (too few free pages, a sequence past
-    `pages.max_len`) changes nothing and records ERR_PAGES (`device_status`)."""
+    `pages.max_len`) changes nothing and records ERR_PAGES (`device_status`); `kv_append` then takes no rows of
+    these sequences until a call for them is met (tokens of 0 are enough) or they are freed."""
     L.calls().kv_reserve(pages.handle, seqs, tokens)
 
 

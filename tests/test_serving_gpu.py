@@ -49,3 +49,44 @@ def test_many_items_key_by_key(hd):
     got = ops.attention_pages(q, c, 0, 12, starts_of(counts), max_q=30)
     assert ops.device_status() == 0
     check(got, *pages_want(q, c, 0, 12, counts, range(len(lens)), True, hd**-0.5))
+
+
+# ------------------------------------------------------------------------------ a reservation that is refused
+
+
+def test_append_after_a_refused_reservation():
+    """The pool runs out: what the sequences hold (a part-filled page, whole pages shared by a fork) stays as it was, through
+    every layer's append, until a later reservation is met."""
+    from so101_smolvla_edge_b200 import _lib as L
+    from so101_smolvla_edge_b200 import ops
+    from so101_smolvla_edge_b200.pages import KvPages
+
+    c = KvPages(2, 6, 2, 64, 4, 128, 16)
+    x = torch.randn(64, 256, device="cuda", generator=torch.Generator("cuda").manual_seed(221)).to(torch.bfloat16)
+
+    def append(seqs, counts):
+        rows = x[: sum(counts)] * (4.0 if sum(counts) < 4 else 1.0)  # larger ones: they would raise the scales
+        for layer in range(2):
+            ops.kv_append(c, layer, rows[:, :128], rows[:, 128:], starts_of(counts), ints(seqs), max_new=max(counts))
+
+    ops.kv_reserve(c, ints([0, 2]), ints([32, 21]))  # two pages that a fork shares, and one and a part
+    append([0, 2], [32, 21])
+    ops.kv_fork(c, ints([0]), ints([1]))
+    ops.kv_reserve(c, ints([3]), ints([30]))
+    append([3], [30])  # all six pages are in use
+    assert ops.device_status() == 0
+    state = (c.k, c.v, c.k_scale, c.v_scale, c.table, c.lengths, c.refs)
+    before = [t.clone() for t in state]
+    ops.kv_reserve(c, ints([1, 2, 3]), ints([1, 1, 1]))  # sequence 1 needs a page
+    append([1, 2, 3], [1, 1, 1])
+    assert all(torch.equal(t, b) for t, b in zip(state, before))
+    assert ops.device_status() == L.ERR_PAGES
+    L.lib().so101_clear_device_status()
+    ops.kv_free(c, ints([3]))
+    ops.kv_reserve(c, ints([1, 2, 3]), ints([1, 1, 1]))
+    append([1, 2, 3], [1, 1, 1])
+    assert ops.device_status() == 0 and c.lengths.tolist() == [32, 33, 22, 1]
+    for s in (1, 2, 3):
+        k, _ = ops.kv_read(c, 1, ints([0, 1]), 1, ints([s]), first=ints([int(c.lengths[s]) - 1]))
+        want = x[s - 1 : s, :128] * 4.0
+        assert (k.float() - want.float()).abs().max() <= want.float().abs().max() / 63.5
