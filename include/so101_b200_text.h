@@ -93,9 +93,9 @@ SO101_API int so101_attention_pages(const void* q, int64_t ldq, void* o, int64_t
                                     cudaStream_t stream);
 
 /* lengths[seqs[i]] += tokens[i], taking the lowest free pages in the order of the list. If any
- * sequence would pass max_pages * page tokens or the pages do not suffice, nothing changes,
- * so101_kv_append takes no rows of these sequences until a call for them is met, and
- * SO101_ERR_PAGES is recorded. The sequences of a call are distinct. */
+ * sequence would pass max_pages * page tokens, is named twice, or the pages do not suffice, nothing
+ * changes, so101_kv_append takes no rows of these sequences until a call for them is met, and
+ * SO101_ERR_PAGES is recorded. */
 SO101_API int so101_kv_reserve(const so101_kv_pages* c, const int* seqs, const int* tokens, int n,
                                cudaStream_t stream);
 

@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_reserve_kernel(const ListA
         bad = 1;
       else
         need = min(pages_for(c, len + add) - pages_for(c, len), c.n_pages + 1);  // the sums stay in 32 bits
+      if (seq >= 0 && seq < c.max_seqs) s.place[seq] = i;
     }
     int here;
     const int off = block_scan(need, here, warp_sums);
@@ -125,8 +126,13 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_reserve_kernel(const ListA
     if (here > c.n_pages) bad = 1;
   }
   __syncthreads();
+  // a sequence named twice: one of its entries finds the other's number (their lengths and pages would be worked out
+  // apart and written over one another, past the end of the table row where both fit only alone)
+  bool twice = false;
+  for (int i = threadIdx.x; i < g.n; i += kPlanThreads)
+    if (g.a[i] >= 0 && g.a[i] < c.max_seqs && s.place[g.a[i]] != i) twice = true;
   const bool enough = !bad && want <= c.n_pages && free_pages(c, want, s.src, warp_sums, first);
-  if (!enough) {
+  if (__syncthreads_or(twice) || !enough) {
     if (threadIdx.x == 0) record_error(g.status, SO101_ERR_PAGES);
     // the lengths stay, so what is appended next would land on older tokens: kv_append leaves these sequences alone
     for (int i = threadIdx.x; i < g.n; i += kPlanThreads)

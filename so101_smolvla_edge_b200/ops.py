@@ -581,8 +581,8 @@ def attention_pages(
 
 def kv_reserve(pages: KvPages, seqs: torch.Tensor, tokens: torch.Tensor) -> None:
     """Sequence seqs[i] grows by tokens[i] (int32, on the device): its length now, its pages from the
-    lowest free ones. The sequences are distinct. A call that cannot be met (too few free pages, a sequence past
-    `pages.max_len`) changes nothing and records ERR_PAGES (`device_status`); `kv_append` then takes no rows of
+    lowest free ones. A call that cannot be met (too few free pages, a sequence past
+    `pages.max_len` or named twice) changes nothing and records ERR_PAGES (`device_status`); `kv_append` then takes no rows of
     these sequences until a call for them is met (tokens of 0 are enough) or they are freed."""
     L.calls().kv_reserve(pages.handle, seqs, tokens)
 

@@ -90,3 +90,23 @@ def test_append_after_a_refused_reservation():
         k, _ = ops.kv_read(c, 1, ints([0, 1]), 1, ints([s]), first=ints([int(c.lengths[s]) - 1]))
         want = x[s - 1 : s, :128] * 4.0
         assert (k.float() - want.float()).abs().max() <= want.float().abs().max() / 63.5
+
+
+@pytest.mark.parametrize("n", [4, 900])
+def test_reserve_with_a_sequence_named_twice(n):
+    """Each entry alone would fit, both together would pass the table row's end: nothing changes."""
+    from so101_smolvla_edge_b200 import _lib as L
+    from so101_smolvla_edge_b200 import ops
+    from so101_smolvla_edge_b200.pages import KvPages
+
+    c = KvPages(1, 2 * n + 8, 1, 64, n, 64, 16)
+    ops.kv_reserve(c, ints([n - 1]), ints([20]))
+    state = (c.table, c.lengths, c.refs)
+    before = [t.clone() for t in state]
+    others = list(range(n - 2))
+    ops.kv_reserve(c, ints([n - 1, *others, n - 1]), ints([40, *[1] * (n - 2), 40]))
+    assert ops.device_status() == L.ERR_PAGES
+    L.lib().so101_clear_device_status()
+    assert all(torch.equal(t, b) for t, b in zip(state, before))
+    ops.kv_reserve(c, ints([n - 1, *others]), ints([40, *[1] * (n - 2)]))
+    assert ops.device_status() == 0 and c.lengths.tolist() == [1] * (n - 2) + [0, 60]
