@@ -58,9 +58,12 @@ class TextTower:
         return self.cos[at], self.sin[at]
 
     def _grow(self, seqs: list[int], counts: list[int]) -> torch.Tensor:
-        """Pages for `counts` more tokens; the packed starts."""
-        ids = self._ints(seqs)
-        ops.kv_reserve(self.pages, ids, self._ints(counts))
+        """Pages for `counts` more tokens; the sequences' numbers on the device. A sequence that a refused call (of
+        which only `check` tells the host) left shorter than this object counts asks for more than there can be, so that the
+        calls after it are refused too, and nothing is cached at a place that is not its own."""
+        ids, held = self._ints(seqs), self._ints([self.lengths[s] for s in seqs])
+        behind = self.pages.lengths[ids] != held
+        ops.kv_reserve(self.pages, ids, torch.add(self._ints(counts), behind, alpha=1 << 30))
         for s, n in zip(seqs, counts):
             self.lengths[s] += n
         return ids
@@ -137,9 +140,15 @@ class TextTower:
         ops.kv_compact(self.pages)
 
     def check(self) -> None:
-        """Raise if a call since the last check could not be met (too few free pages): the cache then stands as
-        before that call, but this object's own count of lengths does not. Reads the device: not once per token."""
-        L.check(ops.device_status(), "TextTower")
+        """Raise if a call since the last check could not be met (too few free pages). The cache then stands as before
+        that call, later calls of its sequences were refused with it (what all of them returned is void), and this
+        object counts the lengths that the cache has. Waits for the device: not once per token."""
+        torch.cuda.current_stream(self.dev).synchronize()
+        status = ops.device_status()
+        if status != L.OK:
+            L.lib().so101_clear_device_status()
+            self.lengths = self.pages.lengths.tolist()
+            L.check(status, "TextTower")
 
     def cached(self, layer: int, seq: int) -> tuple[torch.Tensor, torch.Tensor]:
         """A sequence's cached keys (rotated) and values of one layer, as bf16 rows: what an expert layer that

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from test_text_gpu import cache, check, ints, pages_want, queries, starts_of
+from test_text_tower_gpu import TOKEN, bundle, off, plain  # noqa: F401 (bundle: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +111,40 @@ def test_reserve_with_a_sequence_named_twice(n):
     assert all(torch.equal(t, b) for t, b in zip(state, before))
     ops.kv_reserve(c, ints([n - 1, *others]), ints([40, *[1] * (n - 2)]))
     assert ops.device_status() == 0 and c.lengths.tolist() == [1] * (n - 2) + [0, 60]
+
+
+# ------------------------------------------------------------------------------------------- the text tower
+
+
+def test_tower_goes_on_after_the_pool_ran_out(bundle):  # noqa: F811
+    """Steps that find no page leave the cache as it is, those after them too; check says so once and sets the counts
+    right, and the sequences go on where they stood."""
+    from so101_smolvla_edge_b200 import _lib as L
+    from so101_smolvla_edge_b200.text_tower import TextTower
+
+    g = torch.Generator().manual_seed(231)
+    dim = bundle.spec.text_dim
+    tower = TextTower(bundle, n_pages=6, max_seqs=6, max_len=128, page=32)
+    text = {q: torch.randn(n, dim, generator=g) for q, n in ((0, 64), (1, 40))}
+    tower.prompt(torch.cat(list(text.values())).cuda(), [64, 40], [0, 1])
+    tower.fork([0, 1], [2, 3])  # 2 shares both pages of 0; 3 copies a part: five pages
+    text[2], text[3] = text[0], text[1]
+    tower.prompt(torch.randn(3, dim, generator=g).cuda(), [3], [4])  # the sixth
+    tower.check()
+    pages = tower.pages
+    state = [t.clone() for t in (pages.k, pages.v, pages.k_scale, pages.v_scale, pages.table, pages.lengths, pages.refs)]
+    for seqs in ([0, 1, 3], [1, 3], [2], [1]):  # 0 and 2 need a page; 1 and 3 do not, but went along with 0
+        tower.step(5.0 * torch.randn(len(seqs), dim, generator=g).cuda(), seqs)
+    tower.fork([1], [5])
+    with pytest.raises(L.KernelError):
+        tower.check()
+    for t, was in zip((pages.k, pages.v, pages.k_scale, pages.v_scale, pages.table, pages.lengths, pages.refs), state):
+        assert torch.equal(t, was)
+    tower.check()
+    assert tower.lengths == pages.lengths.tolist() == [64, 40, 64, 40, 3, 0]
+    tower.free([4])
+    rows = torch.randn(3, dim, generator=g)
+    got = tower.step(rows.cuda(), [2, 1, 3])
+    tower.check()
+    for i, q in enumerate((2, 1, 3)):
+        assert off(got[i], plain(bundle, torch.cat([text[q], rows[i : i + 1]]))[-1]) <= TOKEN
