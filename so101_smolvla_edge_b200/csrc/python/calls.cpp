@@ -14,7 +14,9 @@
 
 #include <cstdarg>
 #include <map>
+#include <mutex>
 #include <utility>
+#include <vector>
 
 #include "../../../include/so101_b200_text.h"
 
@@ -159,7 +161,69 @@ int64_t entries(int64_t n_starts, int64_t n_seqs, int64_t rows) {
   return n;
 }
 
+// What a graph under capture uses: (capture id, stream) -> its workspace. The graph may be replayed beside eager calls on its
+// capture stream and beside other graphs captured there, so it has partials and tickets of its own, which it clears
+// at its start and which live as long as it does (a CUDA user object holds them). The object's destructor may run on
+// a thread of the driver's and make no CUDA calls: it hands them to the next call here.
+using CaptureKey = std::pair<unsigned long long, int64_t>;
+struct Held {
+  at::Tensor memory;
+  CaptureKey key;
+};
+std::map<CaptureKey, Space> g_captured;  // under the interpreter lock, as g_spaces
+std::mutex g_ended_lock;
+std::vector<Held*> g_ended;
+
+void CUDART_CB graph_ended(void* held) {
+  const std::lock_guard<std::mutex> lock(g_ended_lock);
+  g_ended.push_back(static_cast<Held*>(held));
+}
+
+void clear_ended() {
+  std::vector<Held*> ended;
+  {
+    const std::lock_guard<std::mutex> lock(g_ended_lock);
+    ended.swap(g_ended);
+  }
+  for (Held* h : ended) {
+    g_captured.erase(h->key);
+    delete h;
+  }
+}
+
+constexpr int64_t kSpaceBytes = int64_t(40) << 20, kSpaceTickets = 1184;
+
+const Space& captured_space(c10::Device dev, cudaStream_t stream, unsigned long long id, cudaGraph_t graph) {
+  const CaptureKey key(id, reinterpret_cast<int64_t>(stream));
+  auto it = g_captured.find(key);
+  if (it != g_captured.end()) return it->second;
+  const auto bytes = at::TensorOptions().dtype(at::kByte).device(dev);
+  const at::Tensor memory = at::empty({kSpaceBytes + kSpaceTickets * 4}, bytes);
+  memory.narrow(0, kSpaceBytes, kSpaceTickets * 4).zero_();
+  Held* held = new Held{memory, key};
+  cudaUserObject_t object;
+  cudaError_t e = cudaUserObjectCreate(&object, held, graph_ended, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) {
+    delete held;
+  } else {
+    e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+  }
+  if (e != cudaSuccess) {
+    PyErr_Format(PyExc_RuntimeError, "a workspace for the graph under capture: %s", cudaGetErrorString(e));
+    throw Raised{};
+  }
+  char* at = static_cast<char*>(memory.data_ptr());
+  return g_captured[key] = Space{at, kSpaceBytes, reinterpret_cast<int*>(at + kSpaceBytes), kSpaceTickets};
+}
+
 const Space& space(c10::Device dev, cudaStream_t stream) {
+  clear_ended();
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo(stream, &capture, &id, &graph) != cudaSuccess) cudaGetLastError();  // the launch will say
+  else if (capture == cudaStreamCaptureStatusActive) return captured_space(dev, stream, id, graph);
   const std::pair<int, int64_t> key(dev.index(), reinterpret_cast<int64_t>(stream));
   auto it = g_spaces.find(key);
   if (it == g_spaces.end()) {

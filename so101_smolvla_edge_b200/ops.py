@@ -480,8 +480,8 @@ _PAGES_WS: dict[tuple[int, int], Workspace] = {}
 
 def pages_workspace(device: int, stream: int) -> Workspace:
     """The partial results of `attention_pages` on one stream of a device (calls on several streams
-    overlap, so each has its own). Made by the first call on the stream: make that call before a CUDA graph
-    is captured there."""
+    overlap, so each has its own). Made by the first call on the stream. A graph under capture does not use
+    it: it gets a workspace of its own, and keeps that until it is destroyed."""
     ws = _PAGES_WS.get((device, stream))
     if ws is None:
         ws = _PAGES_WS[device, stream] = Workspace(torch.device("cuda", device), nbytes=40 << 20)

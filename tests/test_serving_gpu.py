@@ -148,3 +148,96 @@ def test_tower_goes_on_after_the_pool_ran_out(bundle):  # noqa: F811
     tower.check()
     for i, q in enumerate((2, 1, 3)):
         assert off(got[i], plain(bundle, torch.cat([text[q], rows[i : i + 1]]))[-1]) <= TOKEN
+
+
+# ------------------------------------------------------------------------------------------ graphs of attention
+
+
+def attention_graphs(n):
+    """Graphs of single tokens over long sequences (read in parts, so that partials and tickets are in use), captured
+    on torch's own capture stream without a call before them, each with a cache, queries and a result of its own."""
+    from so101_smolvla_edge_b200 import ops
+
+    out = []
+    for i in range(n):
+        c = cache([4000 + 700 * i, 9000], 2, 64, 64, seed=241 + i)
+        q = queries(2, 6, 64, seed=251 + i)
+        y = torch.empty(2, 384, dtype=torch.bfloat16, device="cuda")
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(8):
+                ops.attention_pages(q, c, 0, 6, out=y)
+        out.append((g, c, q, y))
+    return out
+
+
+def test_graphs_captured_on_one_stream_replayed_on_several():
+    from so101_smolvla_edge_b200 import ops
+
+    graphs = attention_graphs(4)
+    want = [pages_want(q, c, 0, 6, [1, 1], [0, 1], True, 0.125) for _, c, q, _ in graphs]
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (g, *_), s in reversed(list(zip(graphs, streams))):  # the first captured is not the first replayed
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = ops.attention_pages(graphs[0][2], graphs[0][1], 0, 6)
+    torch.cuda.synchronize()
+    for (_, _, _, y), w in zip(graphs, want):
+        check(y, *w)
+    check(eager, *want[0])
+    assert ops.device_status() == 0
+
+
+def test_a_graph_beside_eager_calls_on_its_capture_stream():
+    from so101_smolvla_edge_b200 import ops
+
+    c = cache([9000, 5000], 2, 64, 64, seed=261)
+    q = queries(2, 6, 64, seed=262)
+    want = pages_want(q, c, 0, 6, [1, 1], [0, 1], True, 0.125)
+    y = torch.empty(2, 384, dtype=torch.bfloat16, device="cuda")
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        for _ in range(8):
+            ops.attention_pages(q, c, 0, 6, out=y)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(t):
+            g.replay()
+        with torch.cuda.stream(s):
+            got += [ops.attention_pages(q, c, 0, 6) for _ in range(4)]
+    torch.cuda.synchronize()
+    check(y, *want)
+    assert all(torch.equal(x, y) for x in got)
+    assert ops.device_status() == 0
+
+
+def test_a_graphs_workspace_goes_with_it():
+    import gc
+    import time
+
+    from so101_smolvla_edge_b200 import ops
+
+    c, q = cache([9000], 2, 64, 64, seed=271), queries(1, 6, 64, seed=272)
+    attention_graphs(1)  # what a first capture leaves for good
+    ops.attention_pages(q, c, 0, 6)
+    gc.collect()
+    torch.cuda.synchronize()
+    time.sleep(0.5)  # the driver may say a little later that a graph is gone
+    ops.attention_pages(q, c, 0, 6)
+    before = torch.cuda.memory_allocated()
+    graphs = attention_graphs(3)
+    assert torch.cuda.memory_allocated() >= before + 3 * (40 << 20)
+    del graphs
+    gc.collect()
+    for _ in range(100):
+        ops.attention_pages(q, c, 0, 6)
+        if torch.cuda.memory_allocated() <= before:
+            break
+        time.sleep(0.02)
+    assert torch.cuda.memory_allocated() <= before
