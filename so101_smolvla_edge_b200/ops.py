@@ -21,6 +21,7 @@ Preconditions the kernels cannot meet raise ValueError, as the reference's wrapp
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -476,17 +477,22 @@ def set_pdl(enable: bool) -> None:
 
 
 _PAGES_WS: dict[tuple[int, int], Workspace] = {}
+_PAGES_WS_LOCK = threading.RLock()
 
 
 def pages_workspace(device: int, stream: int) -> Workspace:
     """The partial results of `attention_pages` on one stream of a device (calls on several streams
     overlap, so each has its own). Made by the first call on the stream. A graph under capture does not use
     it: it gets a workspace of its own, and keeps that until it is destroyed."""
-    ws = _PAGES_WS.get((device, stream))
-    if ws is None:
-        ws = _PAGES_WS[device, stream] = Workspace(torch.device("cuda", device), nbytes=40 << 20)
-        L.calls().add_workspace(device, stream, ws.partials.data_ptr(), ws.nbytes, ws.tickets.data_ptr(), ws.tickets.numel())
-    return ws
+    # found, made and registered by one thread at a time (allocating lets other threads run): the arrays that are
+    # registered are the ones kept
+    with _PAGES_WS_LOCK:
+        ws = _PAGES_WS.get((device, stream))
+        if ws is None:
+            ws = Workspace(torch.device("cuda", device), nbytes=40 << 20)
+            L.calls().add_workspace(device, stream, ws.partials.data_ptr(), ws.nbytes, ws.tickets.data_ptr(), ws.tickets.numel())
+            _PAGES_WS[device, stream] = ws
+        return ws
 
 
 # The serving operators check their tensors and call the C ABI in one native step (csrc/python/calls.cpp).
