@@ -101,10 +101,17 @@ __device__ __forceinline__ int pt_seen(const PtItem& it, int tok, int causal) {
   return causal ? max(0, min(it.len, it.len - it.n_q + tok + 1)) : it.len;
 }
 
+__device__ __forceinline__ uint32_t timer_low() {  // (4.3 s around)
+  uint32_t t;
+  asm volatile("mov.u32 %0, %globaltimer_lo;" : "=r"(t));
+  return t;
+}
+
 // Row r of the item over the item's keys in fp32, key by key, by a whole warp (lane l: dims l, l + 32, ...):
-// o / l, and the logarithm of l in m (-infinity where it sees none).
+// o / l, and the logarithm of l in m (-infinity where it sees none). The time goes to `alive` every 256 keys.
 template <int HD>
-__device__ __forceinline__ void pt_row_alone(const PagesArgs& a, const PtItem& it, int r, float (&o)[HD / 32], float& m) {
+__device__ __forceinline__ void pt_row_alone(const PagesArgs& a, const PtItem& it, int r, float (&o)[HD / 32], float& m,
+                                             uint32_t* alive) {
   const KvPages& c = a.c;
   const int lane = threadIdx.x & 31;
   int tok, head;
@@ -128,6 +135,7 @@ __device__ __forceinline__ void pt_row_alone(const PagesArgs& a, const PtItem& i
   const int end = min(pt_seen(it, tok, a.causal), it.to * kPtKeys);
   const int* table = c.table + static_cast<long long>(it.seq) * c.max_pages;
   for (int j = it.from * kPtKeys; j < end; ++j) {
+    if (lane == 0 && j % 256 == 0) *reinterpret_cast<volatile uint32_t*>(alive) = timer_low();
     const int id = table[j / c.page];
     if (id < 0 || id >= c.n_pages) {
       record_error(a.status, SO101_ERR_PAGES);
@@ -170,15 +178,24 @@ __device__ __forceinline__ void transpose4(uint4 (&y)[4]) {
   swap(y[1], y[3], 2);
 }
 
-// As mbar_wait, counting instead of timing, in fewer instructions.
-__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, int* status) {
-  uint32_t i = 0;
+// As mbar_wait (2 s of the timer), but not while the time in `alive` is younger than that: items that go key by key note
+// it there, and can hold the others up for longer. (The differences are of 32 bits, 4.3 s: at some time in each turn
+// both are past the limit. The timer is left alone in short waits: 39.1 us for 64 chunks of 50 tokens, 39.6 with it
+// looked at every 256 polls in a loop that tells the first look by its number, 38.6 with polls counted and no timer.)
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, int* status, const uint32_t* alive) {
+  uint32_t t0 = 0;
 #pragma unroll 1
-  while (!mbar_try_wait(bar, parity))
-    if (++i == 1u << 23) {
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+    if (i != 4096u) continue;
+    i = 0;
+    const uint32_t other = *reinterpret_cast<const volatile uint32_t*>(alive), now = timer_low();
+    if (t0 == 0u) {
+      t0 = now | 1u;
+    } else if (now - t0 > kWaitLimitNs && now - other > kWaitLimitNs) {
       record_error(status, SO101_ERR_TIMEOUT);
       return false;
     }
+  }
   return true;
 }
 
@@ -213,7 +230,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
   uint64_t* o_free = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
   int* last = reinterpret_cast<int*>(tmem_slot + 1);  // [8] whether two warps' part came last
-  static_assert(kPtItems * sizeof(PtItem) + (2 * kPtItems + 4 + 6 + 8 + 10) * 8 + 36 <= 1024, "barrier region");
+  uint32_t* alive = reinterpret_cast<uint32_t*>(last + 8);  // when a warp last went on key by key
+  static_assert(kPtItems * sizeof(PtItem) + (2 * kPtItems + 4 + 6 + 8 + 10) * 8 + 40 <= 1024, "barrier region");
   float* factors = reinterpret_cast<float*>(smem + Cfg::kOffFactor);
   float* scales = reinterpret_cast<float*>(smem + Cfg::kOffScale);
 
@@ -245,6 +263,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
       mbar_init(&o_full[lane], 1);
       mbar_init(&o_free[lane], 8);
     }
+    if (lane == 0) *alive = timer_low();
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -261,7 +280,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
   __syncthreads();
 
   auto wait = [&](uint64_t* b, int n) {  // the n-th use (from 0) of a barrier; the same outcome for the whole warp
-    return __all_sync(0xffffffffu, pt_wait(b, static_cast<uint32_t>(n) & 1u, a.status));
+    return __all_sync(0xffffffffu, pt_wait(b, static_cast<uint32_t>(n) & 1u, a.status, alive));
   };
   auto item_at = [&](int i) {
     PtItem it = {};
@@ -751,7 +770,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
         for (int x = hf; x < min(32, it.rows - g * kPtRows - quad * 32); x += 2) {
           const int r = g * kPtRows + quad * 32 + x;
           float o[HD / 32], top;
-          pt_row_alone<HD>(a, it, r, o, top);
+          pt_row_alone<HD>(a, it, r, o, top, alive);
           int tok, head;
           pt_row(a, it, r, tok, head);
           float* mine = slot_at(it.cta_first + it.part, it.part);

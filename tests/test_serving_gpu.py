@@ -52,6 +52,28 @@ def test_many_items_key_by_key(hd):
     check(got, *pages_want(q, c, 0, 12, counts, range(len(lens)), True, hd**-0.5))
 
 
+def test_long_items_key_by_key_hold_nobody_up():
+    """Several items of 131072 keys that go key by key on every CTA (seconds of them), ordinary ones behind them: whoever waits
+    for those goes on waiting. All sequences share the pages of two."""
+    from so101_smolvla_edge_b200 import ops
+
+    long, short, n, heads = 131072, 300, 148, 16
+    lens = ([long] * 3 + [short]) * n
+    base = cache([long, short], 1, 64, 64, seed=215)
+    base.v_scale[:, base.table[0, : long // 64].long()] *= 1.5
+    c = type(base).adopt(base.k, base.v, base.k_scale, base.v_scale, base.table[[0, 0, 0, 1] * n].contiguous(), ints(lens), base.refs)
+    q = queries(2 * 16, heads, 64, seed=216)
+    counts = [16] * len(lens)
+    rows = torch.cat([q[:16].repeat(3, 1), q[16:]]).repeat(n, 1)
+    got = ops.attention_pages(rows, c, 0, heads, starts_of(counts), max_q=16)
+    assert ops.device_status() == 0
+    want, tol = pages_want(q, base, 0, heads, [16, 16], [0, 1], True, 0.125)
+    got = got.reshape(n, 64, -1)
+    check(got[:, 48:], want[16:].expand(n, -1, -1), tol[16:])
+    for i in range(3):
+        check(got[:, 16 * i : 16 * i + 16], want[:16].expand(n, -1, -1), tol[:16])
+
+
 # ------------------------------------------------------------------------------ a reservation that is refused
 
 
