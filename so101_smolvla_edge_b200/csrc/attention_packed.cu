@@ -342,6 +342,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       }
       const uint64_t keep = policy_evict_normal();
       int t = 0;  // this CTA's key tiles so far (ring slot and phase)
+      int k_loads = 0, v_loads = 0;
       bool ok = true;
       for (int i = 0; ok; ++i) {
         const PackedItem it = item_at(i);
@@ -356,15 +357,21 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
               tma_load_2d(smem + Cfg::kOffK + st * Cfg::kStage + h * Cfg::kKTile, &tm_k, &k_full[st],
                           it.kvh * HD + 64 * h, it.start + j * kKeys, keep);
           }
-          if (ok && t >= kStages) ok = wait(&v_empty[st], t / kStages - 1);
+          if (!ok) break;
+          k_loads = t + 1;
+          if (t >= kStages) ok = wait(&v_empty[st], t / kStages - 1);
           if (ok && elect_one()) {
             mbar_arrive_expect_tx(&v_full[st], Cfg::kStage);
             for (int h = 0; h < Cfg::kHalves; ++h)
               tma_load_2d(smem + Cfg::kOffV + st * Cfg::kStage + h * Cfg::kKTile, &tm_v, &v_full[st],
                           it.kvh * HD + 64 * h, it.start + j * kKeys, keep);
           }
+          if (ok) v_loads = t + 1;
         }
       }
+      // copies in flight land before the CTA ends, also where a wait ran out
+      for (int n = max(0, k_loads - kStages); n < k_loads; ++n) wait(&k_full[n % kStages], n / kStages);
+      for (int n = max(0, v_loads - kStages); n < v_loads; ++n) wait(&v_full[n % kStages], n / kStages);
     } else {
       // ---- the MMAs of group g, a warp each (so that neither group waits for the other's softmax),
       // one lane elected at each issue. Two cursors walk the CTA's tiles: S runs ahead of P V by one tile,
@@ -469,6 +476,9 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
         if (ok && !first && s_more) ok = issue_s();
         if (ok && s_more) s_more = step(cs);
       }
+      // MMAs in flight end before TMEM is given back, also where a wait ran out
+      if (cs.own > 0) wait(&s_full[g], cs.own - 1);
+      if (cp.own > 0) wait(&o_full[g], cp.own - 1);
     }
   } else if (warp < 4 + Cfg::kQWarps) {
     // ---- the queries: 16-byte pieces copied into their swizzled places (all of an item's in flight together),

@@ -494,8 +494,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
           if (lane == 0) mbar_arrive(&r_full[st]);
         }
       }
-      if (!ok)  // copies in flight land before the CTA ends
-        for (int n = max(0, t - kRaws); n < t; ++n) wait(&r_full[n % kRaws], n / kRaws);
+      // copies in flight land before the CTA ends, also where a wait ran out
+      for (int n = max(0, t - kRaws); n < t; ++n) wait(&r_full[n % kRaws], n / kRaws);
     } else {
       // ---- the MMAs of group g, a warp each; S runs ahead of P V by one tile (as attention_packed.cu)
       const int g = warp - 1;
@@ -593,6 +593,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) attention_pages_tc_kernel(const
             ok = issue_pv();
         }
       }
+      // MMAs in flight end before TMEM is given back, also where a wait ran out
+      if (cs.own > 0) wait(&s_full[g], cs.own - 1);
+      if (cp.own > 0) wait(&o_full[g], cp.own - 1);
     }
   } else if (warp < 8) {
     // ---- queries (the first item's with the softmax warps, which wait for them)
