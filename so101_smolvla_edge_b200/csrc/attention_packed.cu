@@ -86,7 +86,9 @@ struct PkCfg {
 static_assert(PkCfg<64>::kSmem <= 232448 && PkCfg<128>::kSmem <= 232448, "227 KB of shared memory per CTA");
 
 // One output row in plain fp32 over the keys it may see, by a whole warp: lane l holds dims
-// l, l + 32, ... Only for rows that came out not finite.
+// l, l + 32, ... Only for rows that came out not finite. A warp takes up to 16 of them one after another while the CTA's
+// others wait, for two seconds at most: those are reached at 750000 tokens (heads of 64; 430000 of 128), at 200000 and
+// 130000 with 32 rows a warp and one key at a time.
 template <int HD>
 __device__ __forceinline__ void packed_row_alone(const PackedArgs& a, int start, int tok, int head, int kvh) {
   const int lane = threadIdx.x & 31;
@@ -105,21 +107,40 @@ __device__ __forceinline__ void packed_row_alone(const PackedArgs& a, int start,
     o[i] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
-  for (int j = 0; j <= tok; ++j) {
-    const __nv_bfloat16* kr = a.k + (start + j) * a.ldk + kvh * HD;
-    const __nv_bfloat16* vr = a.v + (start + j) * a.ldv + kvh * HD;
-    float s = 0.f;
+  constexpr int kAt = 256 / HD;  // keys at a time, their loads in flight together
+  for (int j0 = 0; j0 <= tok; j0 += kAt) {
+    float s[kAt];
 #pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(q[i], __bfloat162float(kr[lane + 32 * i]), s);
+    for (int b = 0; b < kAt; ++b) {
+      const __nv_bfloat16* kr = a.k + (start + min(j0 + b, tok)) * a.ldk + kvh * HD;
+      s[b] = 0.f;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= a.scale_log2;
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2f(m - base), p = exp2f(s - base);
+      for (int i = 0; i < N; ++i) s[b] = fmaf(q[i], __bfloat162float(kr[lane + 32 * i]), s[b]);
+    }
+    float mn = m;
+#pragma unroll
+    for (int b = 0; b < kAt; ++b) {
+#pragma unroll
+      for (int d = 16; d; d >>= 1) s[b] += __shfl_xor_sync(0xffffffffu, s[b], d);
+      s[b] = j0 + b <= tok ? s[b] * a.scale_log2 : -INFINITY;
+      mn = fmaxf(mn, s[b]);
+    }
+    const float base = mn == -INFINITY ? 0.f : mn, alpha = exp2f(m - base);
     m = mn;
-    l = l * alpha + p;
+    l *= alpha;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * alpha + p * __bfloat162float(vr[lane + 32 * i]);
+    for (int i = 0; i < N; ++i) o[i] *= alpha;
+#pragma unroll
+    for (int b = 0; b < kAt; ++b) {
+      const __nv_bfloat16* vr = a.v + (start + min(j0 + b, tok)) * a.ldv + kvh * HD;
+      const float p = exp2f(s[b] - base);
+      l += p;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float x = __bfloat162float(vr[lane + 32 * i]);
+        if (j0 + b <= tok) o[i] = fmaf(p, x, o[i]);
+      }
+    }
   }
   __nv_bfloat16* out = a.o + (start + tok) * a.ldo + head * HD;
 #pragma unroll
@@ -826,14 +847,15 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
           if (g * kPkRows + quad * 32 + w < it.rows) *(reinterpret_cast<uint4*>(a.o + to + h) + (lane & 3)) = y[c];
         }
       }
-      // rows that are not finite, again (by the warp of the first half: all of the row)
+      // rows that are not finite, again: whole, every other one by either warp
       if (!ok) worst = 0xFFFFFFFFu;
       worst = max(worst, __float_as_uint(other(__uint_as_float(worst))));
       if (__any_sync(0xffffffffu, worst == 0xFFFFFFFFu)) break;
       unsigned again = __ballot_sync(0xffffffffu, live && worst >= 0x7F800000u);
-      while (again && hf == 0) {
+      for (int n = 0; again; ++n) {
         const int x = __ffs(again) - 1;
         again &= again - 1;
+        if ((n & 1) != hf) continue;
         packed_row_alone<HD>(a, it.start, __shfl_sync(0xffffffffu, tok, x), __shfl_sync(0xffffffffu, head, x), it.kvh);
       }
     }

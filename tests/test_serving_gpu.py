@@ -8,7 +8,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_text_gpu import cache, check, ints, pages_want, queries, starts_of
+from test_text_gpu import attend, cache, check, ints, pages_want, queries, starts_of
 from test_text_tower_gpu import TOKEN, bundle, off, plain  # noqa: F401 (bundle: a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -72,6 +72,24 @@ def test_long_items_key_by_key_hold_nobody_up():
     check(got[:, 48:], want[16:].expand(n, -1, -1), tol[16:])
     for i in range(3):
         check(got[:, 16 * i : 16 * i + 16], want[:16].expand(n, -1, -1), tol[:16])
+
+
+def test_packed_rows_again_in_a_long_prompt():
+    """An infinity in the last values of a long prompt: the rows before it that share its tile are taken again, key by key
+    (seconds of it), while the CTA's other rows wait."""
+    from so101_smolvla_edge_b200 import ops
+
+    n, hd, bad = 420_000, 64, 60
+    x = torch.randn(n, 3 * hd, device="cuda", generator=torch.Generator("cuda").manual_seed(218)).to(torch.bfloat16)
+    q, k, v = x[:, :hd], x[:, hd : 2 * hd], x[:, 2 * hd :]
+    rows = torch.cat([torch.randint(0, n, (200,), generator=torch.Generator().manual_seed(219)), torch.arange(n - 300, n)]).cuda()
+    fine = rows < n - bad
+    want, tol = zip(*(attend(q[r], k, v, r, hd**-0.5, 0.0, 2**-8) for r in rows[fine].split(50)))
+    v[n - bad] = float("inf")
+    got = ops.attention_packed(q, k, v, ints([0, n]), n, 1, 1)
+    assert ops.device_status() == 0
+    check(got[rows[fine]], torch.cat(want), torch.cat(tol))
+    assert not torch.isfinite(got[n - bad :]).any()
 
 
 # ------------------------------------------------------------------------------ a reservation that is refused
