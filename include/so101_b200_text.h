@@ -26,8 +26,9 @@ extern "C" {
  * three (starts: n_seqs + 1 int32, non-decreasing, starts[n_seqs] <= rows; empty sequences are
  * fine); its row r sees its rows 0..r and nothing else, whatever the other rows hold (infinities
  * and NaN included). max_len: at least the longest sequence. cos / sin (rows, hd/2 fp32) rotate q
- * on load in fp32 (NULL: none), kept as two bf16 parts at hd 64 and rounded to bf16 at 128; k comes
- * rotated. scale multiplies q.k. hd 64 or 128; 16-byte aligned bases (cos and sin too) and row strides. Rows outside every sequence are not written. */
+ * on load in fp32 (NULL: none), kept as two bf16 parts; k comes rotated. scale multiplies q.k. hd 64
+ * or 128; 16-byte aligned bases (cos and sin too) and row strides. Rows outside every sequence are
+ * not written. */
 SO101_API int so101_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
                                      int64_t ldv, void* o, int64_t ldo, int64_t rows, const int* starts,
                                      int n_seqs, int64_t max_len, int nq, int nkv, int hd, float scale,

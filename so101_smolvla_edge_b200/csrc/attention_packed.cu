@@ -15,9 +15,10 @@
 //   2-5  the softmax, and O / l to the output rows: two threads per row (TMEM lane)
 // While a group's softmax runs, the tensor pipe works for the other one. TMEM holds S (128 columns), P and O of
 // both groups at head_dim 64; at 128, S and O only, and P takes the place of the S that it came from.
-// Rotated queries are kept in two bf16 parts at head_dim 64 (value and remainder, two MMAs into one S): tensor
-// time is not what bounds it, and the error against 64 bits falls from 2.6e-3 to 1.9e-3 (1.6e-3 is the
-// rounding of the result). At 128 there is no shared memory for the second part: one rounding to bf16.
+// Rotated queries are kept in two bf16 parts (value and remainder, two MMAs into one S): the error against 64 bits falls
+// from 2.6e-3 to 1.9e-3 (1.6e-3 is the rounding of the result). At 128 the second part takes the place of a tile of K and V,
+// which go through one ring of three then: one sequence of 8191 tokens 800 us, 636 with one part (tiles of 64 keys, two of
+// each: 1058); 64 prompts of 113 to 305 150 us, 128 with one part.
 // The row maximum is only raised when a tile exceeds it by more than 2^8 (as in the SigLIP kernel).
 // Keys past the row's own token are masked by their index. Their values still meet P = 0 in the MMA, where an
 // infinity or a NaN in a value the row must not see would make the row NaN, so a row whose result is
@@ -27,6 +28,7 @@
 // S -> maximum -> exponentials -> P V -> next S bounds it, with the issue slots half and the tensor pipe 41 to 55% busy.
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "kv_pages.cuh"
 #include "tc_attn.cuh"
@@ -51,23 +53,31 @@ struct PackedArgs {
 
 constexpr int kPkRows = 128;  // rows per group (MMA M)
 constexpr float kPkStaleMax = 8.f;
-template <int HD>
+// PARTS: bf16 parts of a query that are held (2: it is rotated here, always at head_dim 64).
+template <int HD, int PARTS>
 struct PkCfg {
   static constexpr int kHalves = HD / 64;             // 64-dim (128-byte) tiles of a row
   static constexpr int kKeys = 128;                   // keys per tile
   static constexpr int kQTile = kPkRows * 128;        // 16 KB: 128 rows x 64 dims
   static constexpr int kKTile = kKeys * 128;          // kKeys rows x 64 dims
   static constexpr int kStage = kHalves * kKTile;     // a K or V tile
-  static constexpr int kParts = HD == 64 ? 2 : 1;     // bf16 parts of a rotated query
   static constexpr int kQBufs = HD == 64 ? 2 : 1;     // items whose queries are held
-  static constexpr int kStages = 2;                   // K and V tiles each
-  static constexpr int kQGroup = kParts * kHalves * kQTile;  // a group's queries
+  // K and V tiles: two of each, or, beside two parts of queries of 128 dims, three in one ring that they take in turn
+  static constexpr bool kOneRing = HD == 128 && PARTS == 2;
+  static constexpr int kSlots = kOneRing ? 3 : 4;
+  static constexpr int kBars = kOneRing ? 3 : 2;      // barriers of a kind (K's and V's are the same in one ring)
+  __device__ static constexpr int k_slot(int t) { return kOneRing ? 2 * t % 3 : t % 2; }
+  __device__ static constexpr int k_use(int t) { return kOneRing ? 2 * t / 3 : t / 2; }
+  __device__ static constexpr int v_slot(int t) { return kOneRing ? (2 * t + 1) % 3 : t % 2; }
+  __device__ static constexpr int v_use(int t) { return kOneRing ? (2 * t + 1) / 3 : t / 2; }
+  static constexpr int kQGroup = PARTS * kHalves * kQTile;  // a group's queries
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kQBufs * 2 * kQGroup;
-  static constexpr int kOffV = kOffK + kStages * kStage;
-  static constexpr int kOffSwap = kOffV + kStages * kStage;  // [2][2 groups][2 halves][128] floats between half rows
-  static constexpr int kOffBar = kOffSwap + 4096;
-  static constexpr int kSmem = kOffBar + 768 + 1024;
+  static constexpr int kOffV = kOneRing ? kOffK : kOffK + 2 * kStage;
+  // [2][2 groups][2 halves][128] values between half rows: floats, or their halves where floats do not fit
+  static constexpr int kOffSwap = kOffK + kSlots * kStage;
+  static constexpr int kOffBar = kOffSwap + (kOneRing ? 2048 : 4096);
+  static constexpr int kSmem = kOffBar + 768 + (kOneRing ? 0 : 1024);
   // TMEM columns of a group. head_dim 64: S (128), P (64) and O (64) side by side; 128: S and O (128 each), P in
   // the place of the S that it came from.
   static constexpr bool kAlias = HD == 128;
@@ -75,15 +85,16 @@ struct PkCfg {
   // Warps: four for loads, MMAs and the item list, then the queries', then 16 for the softmax. Registers per thread
   // of each kind: together no more than the threads start with (80 of 768 threads).
   // At head_dim 128 the softmax threads turn the queries that those four bring, between an item's last P and its O
-  // (64 prompts of 113 to 305 tokens, 32 heads on 8: 135 us, 182 with the four turning them); at 64, with two buffers, the
-  // four do (15 heads on 5: 54 us, 55; 64 prompts of 512 120 and 129).
-  static constexpr bool kSoftTurns = HD == 128;
+  // (64 prompts of 113 to 305 tokens, 32 heads on 8, in one part: 135 us, 182 with the four turning them); at 64, with two
+  // buffers, the four do (15 heads on 5: 54 us, 55; 64 prompts of 512 120 and 129).
+  static constexpr bool kSoftTurns = HD == 128 && PARTS == 2;
   static constexpr int kQWarps = 4;
   static constexpr int kThreads = 32 * (4 + kQWarps + 16);
   static constexpr int kRegsLoad = HD == 64 ? 40 : 48, kRegsQuery = HD == 64 ? 72 : 40, kRegsSoft = HD == 64 ? 88 : 96;
   static constexpr int kItemReaders = 1 + 4 + kQWarps + 16;  // reads of each item: loads, MMAs 2 x 2 (S, P V), queries, softmax
 };
-static_assert(PkCfg<64>::kSmem <= 232448 && PkCfg<128>::kSmem <= 232448, "227 KB of shared memory per CTA");
+static_assert(PkCfg<64, 2>::kSmem <= 232448 && PkCfg<128, 1>::kSmem <= 232448 && PkCfg<128, 2>::kSmem <= 232448,
+              "227 KB of shared memory per CTA");
 
 // One output row in plain fp32 over the keys it may see, by a whole warp: lane l holds dims
 // l, l + 32, ... Only for rows that came out not finite. A warp takes up to 16 of them one after another while the CTA's
@@ -250,14 +261,18 @@ struct PackedWalk {
 
 constexpr int kPkItems = 8;           // items that the list in shared memory holds
 
-template <int HD>
-__global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
+template <int HD, int PARTS>
+__global__ void __launch_bounds__(PkCfg<HD, PARTS>::kThreads, 1)
     attention_packed_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                             const PackedArgs a) {
-  using Cfg = PkCfg<HD>;
-  constexpr int kStages = Cfg::kStages, kQBufs = Cfg::kQBufs, kKeys = Cfg::kKeys;
+  using Cfg = PkCfg<HD, PARTS>;
+  constexpr int kBars = Cfg::kBars, kQBufs = Cfg::kQBufs, kKeys = Cfg::kKeys;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if (Cfg::kOneRing && smem != smem_raw) {  // no bytes to spare (dynamic shared memory starts on 1024 bytes here)
+    if (threadIdx.x == 0) record_error(a.status, SO101_ERR_LAUNCH);
+    return;
+  }
   PackedItem* items = reinterpret_cast<PackedItem*>(smem + Cfg::kOffBar);
   uint64_t* item_full = reinterpret_cast<uint64_t*>(items + kPkItems);  // [kPkItems]
   uint64_t* item_empty = item_full + kPkItems;                         // [kPkItems] read by every warp
@@ -265,11 +280,11 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
   uint64_t* q_raw = q_full + 2 * kQBufs;     // [kQBufs] an item's queries are there, to be turned
   uint64_t* q_empty = q_raw + kQBufs;        // [kQBufs] both groups' S MMAs have read them
   uint64_t* q_first = q_empty + kQBufs;      // [1] the first item's queries are written
-  uint64_t* k_full = q_first + 1;            // [kStages]
-  uint64_t* k_empty = k_full + kStages;      // [kStages]
-  uint64_t* v_full = k_empty + kStages;      // [kStages]
-  uint64_t* v_empty = v_full + kStages;      // [kStages]
-  uint64_t* s_full = v_empty + kStages;      // [2] per group: S written
+  uint64_t* k_full = q_first + 1;            // [kBars]
+  uint64_t* k_empty = k_full + kBars;        // [kBars]
+  uint64_t* v_full = Cfg::kOneRing ? k_full : k_empty + kBars;  // [kBars]
+  uint64_t* v_empty = Cfg::kOneRing ? k_empty : v_full + kBars;  // [kBars]
+  uint64_t* s_full = v_empty + kBars;        // [2] per group: S written
   uint64_t* s_free = s_full + 2;             // [2] S read into registers (head_dim 64)
   uint64_t* p_full = s_free + 2;             // [2] P written, O rescaled
   // [2] P V added to O; everyone waits for each of them (a phase's parity only tells it from its neighbours)
@@ -293,9 +308,11 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       mbar_init(&q_empty[lane], 2);
     }
     if (lane == 0) mbar_init(q_first, 16);
-    if (lane < kStages) {
+    if (lane < kBars) {
       mbar_init(&k_full[lane], 1);
       mbar_init(&k_empty[lane], 2);
+    }
+    if (lane < kBars && !Cfg::kOneRing) {
       mbar_init(&v_full[lane], 1);
       mbar_init(&v_empty[lane], 2);
     }
@@ -323,7 +340,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
   grid_dep_launch();
   grid_dep_wait();
 
-  const bool parted = Cfg::kParts == 2 && a.cos != nullptr;  // a second part of the queries
+  const bool parted = PARTS == 2 && a.cos != nullptr;  // a second part of the queries
   // waits whose outcome is the same for the whole warp; the n-th use (from 0) of a barrier
   auto wait = [&](uint64_t* b, int n) {
     return __all_sync(0xffffffffu, mbar_wait(b, static_cast<uint32_t>(n) & 1u, a.status));
@@ -370,29 +387,34 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
         if (it.rows == 0) break;
         const int n_tiles = it.all_tiles();
         for (int j = 0; j < n_tiles && ok; ++j, ++t) {
-          const int st = t % kStages;
-          if (t >= kStages) ok = wait(&k_empty[st], t / kStages - 1);
+          const int ks = Cfg::k_slot(t), vs = Cfg::v_slot(t);
+          if (Cfg::k_use(t) > 0) ok = wait(&k_empty[ks], Cfg::k_use(t) - 1);
           if (ok && elect_one()) {
-            mbar_arrive_expect_tx(&k_full[st], Cfg::kStage);
+            mbar_arrive_expect_tx(&k_full[ks], Cfg::kStage);
             for (int h = 0; h < Cfg::kHalves; ++h)
-              tma_load_2d(smem + Cfg::kOffK + st * Cfg::kStage + h * Cfg::kKTile, &tm_k, &k_full[st],
+              tma_load_2d(smem + Cfg::kOffK + ks * Cfg::kStage + h * Cfg::kKTile, &tm_k, &k_full[ks],
                           it.kvh * HD + 64 * h, it.start + j * kKeys, keep);
           }
           if (!ok) break;
           k_loads = t + 1;
-          if (t >= kStages) ok = wait(&v_empty[st], t / kStages - 1);
+          if (Cfg::v_use(t) > 0) ok = wait(&v_empty[vs], Cfg::v_use(t) - 1);
           if (ok && elect_one()) {
-            mbar_arrive_expect_tx(&v_full[st], Cfg::kStage);
+            mbar_arrive_expect_tx(&v_full[vs], Cfg::kStage);
             for (int h = 0; h < Cfg::kHalves; ++h)
-              tma_load_2d(smem + Cfg::kOffV + st * Cfg::kStage + h * Cfg::kKTile, &tm_v, &v_full[st],
+              tma_load_2d(smem + Cfg::kOffV + vs * Cfg::kStage + h * Cfg::kKTile, &tm_v, &v_full[vs],
                           it.kvh * HD + 64 * h, it.start + j * kKeys, keep);
           }
           if (ok) v_loads = t + 1;
         }
       }
       // copies in flight land before the CTA ends, also where a wait ran out
-      for (int n = max(0, k_loads - kStages); n < k_loads; ++n) wait(&k_full[n % kStages], n / kStages);
-      for (int n = max(0, v_loads - kStages); n < v_loads; ++n) wait(&v_full[n % kStages], n / kStages);
+      if (Cfg::kOneRing) {
+        const int loads = k_loads + v_loads;  // in turn
+        for (int n = max(0, loads - 3); n < loads; ++n) wait(&k_full[n % 3], n / 3);
+      } else {
+        for (int n = max(0, k_loads - 2); n < k_loads; ++n) wait(&k_full[n % 2], n / 2);
+        for (int n = max(0, v_loads - 2); n < v_loads; ++n) wait(&v_full[n % 2], n / 2);
+      }
     } else {
       // ---- the MMAs of group g, a warp each (so that neither group waits for the other's softmax),
       // one lane elected at each issue. Two cursors walk the CTA's tiles: S runs ahead of P V by one tile,
@@ -420,11 +442,11 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
       };
       // S of the cursor's tile (the K stage freed where the group has no rows for it)
       auto issue_s = [&]() {
-        const int st = cs.t % kStages, qb = cs.item % kQBufs;
+        const int st = Cfg::k_slot(cs.t), qb = cs.item % kQBufs;
         const bool has = cs.j < cs.mine;
         // (q_full[0]'s first use is for item kQBufs)
         const bool queries = cs.j > 0 || (cs.item == 0 ? wait(q_first, 0) : wait(&q_full[2 * qb + g], cs.item / kQBufs - (qb == 0 ? 1 : 0)));
-        if (!queries || !wait(&k_full[st], cs.t / kStages)) return false;
+        if (!queries || !wait(&k_full[st], Cfg::k_use(cs.t))) return false;
         // the S before is in registers; where P took its place, P V has read that
         if (has && cs.own > 0 && !(Cfg::kAlias ? pv_done(cs.own - 1) : wait(&s_free[g], cs.own - 1))) return false;
         tc_fence_after();
@@ -457,9 +479,9 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
         return true;
       };
       auto issue_pv = [&]() {
-        const int st = cp.t % kStages;
+        const int st = Cfg::v_slot(cp.t);
         const bool has = cp.j < cp.mine;
-        if (!wait(&v_full[st], cp.t / kStages) || (has && !wait(&p_full[g], cp.own))) return false;
+        if (!wait(&v_full[st], Cfg::v_use(cp.t)) || (has && !wait(&p_full[g], cp.own))) return false;
         if (has && cp.j == 0 && n_items > 0 && !wait(&o_free[g], n_items - 1)) return false;
         tc_fence_after();
         if (elect_one()) {
@@ -535,7 +557,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
                      : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      if (a.cos && !Cfg::kSoftTurns) {
+      if (PARTS == 2 && a.cos && !Cfg::kSoftTurns) {
         // a lane takes 8 dims (and their partners) of a token at a time, for all its heads; the next token's
         // angles are asked for before this one's are used, the first ones beside the copies
         const int first = real > 0 ? token(row0) : 0, tasks = real > 0 ? (token(row0 + real - 1) - first + 1) * kPairs : 0;
@@ -563,16 +585,16 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
             uint4* u1 = reinterpret_cast<uint4*>(at(r, c));
             uint4* u2 = reinterpret_cast<uint4*>(at(r, c + kPairs));
             uint4 x1 = *u1, x2 = *u2, l1, l2;
-            packed_turn<Cfg::kParts>(x1, x2, l1, l2, cv, sv);
+            packed_turn<PARTS>(x1, x2, l1, l2, cv, sv);
             *u1 = x1;
             *u2 = x2;
-            if (Cfg::kParts == 2) {
+            if (PARTS == 2) {
               *reinterpret_cast<uint4*>(at(r, c) + Cfg::kHalves * Cfg::kQTile) = l1;
               *reinterpret_cast<uint4*>(at(r, c + kPairs) + Cfg::kHalves * Cfg::kQTile) = l2;
             }
           }
         }
-        if (Cfg::kParts == 2)  // the second part of padding rows
+        if (PARTS == 2)  // the second part of padding rows
           for (int p = real * kPieces + lane; p < rows * kPieces; p += 32)
             *reinterpret_cast<uint4*>(at(row0 + p / kPieces, p % kPieces) + Cfg::kHalves * Cfg::kQTile) = make_uint4(0u, 0u, 0u, 0u);
       } else {
@@ -601,16 +623,23 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16) + g * Cfg::kGroupCols;
     const uint32_t s_addr = lane_base + Cfg::kColS + hf * kMine, p_addr = lane_base + Cfg::kColP + hf * (kMine / 2);
     const uint32_t o_addr = lane_base + Cfg::kColO + hf * (HD / 2);  // half of the row's O is this thread's too
-    float* swap = reinterpret_cast<float*>(smem + Cfg::kOffSwap) + g * 256 + rl;  // + 512 per buffer, 128 per half
+    using Swap = typename std::conditional<Cfg::kOneRing, unsigned short, unsigned>::type;
+    Swap* swap = reinterpret_cast<Swap*>(smem + Cfg::kOffSwap) + g * 256 + rl;  // + 512 per buffer, 128 per half
     const float sc = a.scale_log2;
     auto pv_done = [&](int n) { return wait(&o_full[g], n); };  // this group's n-th P V
     int n_swap = 0;
     // what the other half of the row has. The two buffers take turns: a value is read before the next but one is written.
-    auto other = [&](float x) {
-      float* at = swap + (n_swap++ & 1) * 512;
-      at[hf * 128] = x;
+    auto other_bits = [&](unsigned x) -> unsigned {
+      Swap* at = swap + (n_swap++ & 1) * 512;
+      at[hf * 128] = static_cast<Swap>(x);
       asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + quad) : "memory");
       return at[(hf ^ 1) * 128];
+    };
+    auto other = [&](float x) {
+      const unsigned u = __float_as_uint(x);
+      if (!Cfg::kOneRing) return __uint_as_float(other_bits(u));
+      const unsigned high = other_bits(u >> 16);
+      return __uint_as_float(high << 16 | other_bits(u & 0xFFFFu));
     };
     {  // the first item's queries: half of row rl's pairs of pieces
       const PackedItem it = item_at(0, true);
@@ -628,7 +657,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
           if (r < it.rows) {
             x1 = __ldg(qr + c);
             x2 = __ldg(qr + c + kPairs);
-            if (a.cos) {
+            if (PARTS == 2 && a.cos) {
               const long long at = static_cast<long long>(it.start + tok) * (HD / 2) + 8 * c;
               float4 ang[4];
               ang[0] = __ldg(reinterpret_cast<const float4*>(a.cos + at));
@@ -636,7 +665,7 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
               ang[2] = __ldg(reinterpret_cast<const float4*>(a.sin + at));
               ang[3] = __ldg(reinterpret_cast<const float4*>(a.sin + at + 4));
               const float* cv = reinterpret_cast<const float*>(ang);
-              packed_turn<Cfg::kParts>(x1, x2, l1, l2, cv, cv + 8);
+              packed_turn<PARTS>(x1, x2, l1, l2, cv, cv + 8);
             }
           }
           uint8_t* d1 = to + c / 8 * Cfg::kQTile + ((c % 8 ^ (rl & 7)) << 4);
@@ -682,9 +711,11 @@ __global__ void __launch_bounds__(PkCfg<HD>::kThreads, 1)
           uint4* u2 = reinterpret_cast<uint4*>(to + (c + kPairs) / 8 * Cfg::kQTile + (((c + kPairs) % 8 ^ (rl & 7)) << 4));
           uint4 x1 = *u1, x2 = *u2, l1, l2;
           const float* cv = reinterpret_cast<const float*>(ang[z]);
-          packed_turn<Cfg::kParts>(x1, x2, l1, l2, cv, cv + 8);
+          packed_turn<PARTS>(x1, x2, l1, l2, cv, cv + 8);
           *u1 = x1;
           *u2 = x2;
+          *(u1 + Cfg::kHalves * Cfg::kQTile / 16) = l1;
+          *(u2 + Cfg::kHalves * Cfg::kQTile / 16) = l2;
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -894,7 +925,7 @@ int packed_map(CUtensorMap* m, const void* base, long long rows, long long cols,
              : SO101_ERR_ARG;
 }
 
-template <int HD>
+template <int HD, int PARTS>
 int launch_packed(const CUtensorMap& tk, const CUtensorMap& tv, PackedArgs a, cudaStream_t stream) {
   static std::atomic<int> sms[64];
   int dev = 0;
@@ -902,8 +933,8 @@ int launch_packed(const CUtensorMap& tk, const CUtensorMap& tv, PackedArgs a, cu
   if (dev < 0 || dev >= 64) return SO101_ERR_DRIVER;
   int full = sms[dev].load();
   if (!full) {
-    cudaError_t e = cudaFuncSetAttribute(attention_packed_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         PkCfg<HD>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(attention_packed_kernel<HD, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         PkCfg<HD, PARTS>::kSmem);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&full, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return launch_error(e);
     sms[dev].store(full);
@@ -916,7 +947,7 @@ int launch_packed(const CUtensorMap& tk, const CUtensorMap& tv, PackedArgs a, cu
   const int64_t items = (stacked / a.block + part) * a.n_kv;
   if (items > (1 << 30)) return SO101_ERR_ARG;
   const dim3 grid(static_cast<unsigned>(items < full ? items : full));
-  return launch_kernel(attention_packed_kernel<HD>, grid, dim3(PkCfg<HD>::kThreads), PkCfg<HD>::kSmem, stream, tk, tv, a);
+  return launch_kernel(attention_packed_kernel<HD, PARTS>, grid, dim3(PkCfg<HD, PARTS>::kThreads), PkCfg<HD, PARTS>::kSmem, stream, tk, tv, a);
 }
 
 }  // namespace
@@ -963,5 +994,6 @@ extern "C" int so101_attention_packed(const void* q, int64_t ldq, const void* k,
   a.status = status_ptr();
   a.n_kv = nkv;
   a.group_inv = 65536 / a.group + 1;
-  return hd == 64 ? launch_packed<64>(tk, tv, a, stream) : launch_packed<128>(tk, tv, a, stream);
+  if (hd == 64) return launch_packed<64, 2>(tk, tv, a, stream);
+  return cos ? launch_packed<128, 2>(tk, tv, a, stream) : launch_packed<128, 1>(tk, tv, a, stream);
 }

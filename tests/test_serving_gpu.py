@@ -8,7 +8,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_text_gpu import attend, cache, check, ints, pages_want, queries, starts_of
+from test_text_gpu import attend, cache, check, ints, packed_case, pages_want, queries, rope, starts_of, turn
 from test_text_tower_gpu import TOKEN, bundle, off, plain  # noqa: F401 (bundle: a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -90,6 +90,26 @@ def test_packed_rows_again_in_a_long_prompt():
     assert ops.device_status() == 0
     check(got[rows[fine]], torch.cat(want), torch.cat(tol))
     assert not torch.isfinite(got[n - bad :]).any()
+
+
+@pytest.mark.parametrize("lens", [[300, 77, 128], [43] * 90, [1, 700]])
+@pytest.mark.parametrize("heads,kv,hd", [(15, 5, 64), (6, 2, 128), (3, 3, 128)])
+def test_rotated_queries_keep_two_parts(lens, heads, kv, hd):
+    """Scores of tens, where a rotated query rounded to bf16 once would show: what is left of it after two parts is 2^-16
+    of a value (the rest of the tolerance as in test_text_gpu.py)."""
+    from so101_smolvla_edge_b200 import ops
+
+    q, k, v = packed_case(lens, heads, kv, hd, seed=229, big=16.0)
+    cos, sin = rope(torch.cat([torch.arange(n) for n in lens]), hd)
+    got = ops.attention_packed(q, k, v, starts_of(lens), max(lens), heads, kv, cos=cos, sin=sin)
+    qr, at = turn(q.double().reshape(-1, heads, hd), cos, sin), 0
+    for n in lens:
+        for h in range(heads):
+            sl, g = slice(at, at + n), h // (heads // kv) * hd
+            want, tol = attend(qr[sl, h], k[sl, g : g + hd], v[sl, g : g + hd], torch.arange(n, device="cuda"), hd**-0.5, 2**-16, 2**-8)
+            check(got[sl, h * hd : (h + 1) * hd], want, tol)
+        at += n
+    assert ops.device_status() == 0
 
 
 # ------------------------------------------------------------------------------ a reservation that is refused
