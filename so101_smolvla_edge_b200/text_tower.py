@@ -50,23 +50,27 @@ class TextTower:
         self.cos, self.sin = (t.to(self.dev) for t in _rope(torch.arange(self.pages.max_len), s.head_dim, s.rope_wavelength))
         self.lengths = [0] * max_seqs  # the host's own count: what the next positions are
 
-    def _ints(self, x: list[int]) -> torch.Tensor:
-        return torch.tensor(x, dtype=torch.int32, device=self.dev)
+    def _put(self, *lists) -> tuple[torch.Tensor, ...]:
+        """Lists of integers on the device, in one copy from pinned memory that the host does not wait for."""
+        parts = [torch.as_tensor(x, dtype=torch.int32) for x in lists]
+        sizes = [x.numel() for x in parts]
+        host = torch.cat(parts, out=torch.empty(sum(sizes), dtype=torch.int32, pin_memory=True))
+        return host.to(self.dev, non_blocking=True).split(sizes)
 
-    def _angles(self, seqs: list[int], counts: list[int]) -> tuple[torch.Tensor, torch.Tensor]:
-        at = torch.cat([torch.arange(self.lengths[s], self.lengths[s] + n) for s, n in zip(seqs, counts)]).to(self.dev)
-        return self.cos[at], self.sin[at]
-
-    def _grow(self, seqs: list[int], counts: list[int]) -> torch.Tensor:
-        """Pages for `counts` more tokens; the sequences' numbers on the device. A sequence that a refused call (of
-        which only `check` tells the host) left shorter than this object counts asks for more than there can be, so that the
-        calls after it are refused too, and nothing is cached at a place that is not its own."""
-        ids, held = self._ints(seqs), self._ints([self.lengths[s] for s in seqs])
+    def _grow(self, seqs: list[int], counts: list[int]) -> tuple[torch.Tensor, ...]:
+        """Pages for `counts` more tokens. Returns the sequences' numbers, the packed starts and the new tokens' angles, on
+        the device. A sequence that a refused call (of which only `check` tells the host) left shorter than this object
+        counts asks for more than there can be, so that the calls after it are refused too, and nothing is cached at a place
+        that is not its own."""
+        held = [self.lengths[s] for s in seqs]
+        starts = [0, *torch.tensor(counts).cumsum(0).tolist()]
+        at = torch.cat([torch.arange(h, h + n, dtype=torch.int32) for h, n in zip(held, counts)])
+        ids, more, held, starts, at = self._put(seqs, counts, held, starts, at)
         behind = self.pages.lengths[ids] != held
-        ops.kv_reserve(self.pages, ids, torch.add(self._ints(counts), behind, alpha=1 << 30))
+        ops.kv_reserve(self.pages, ids, torch.add(more, behind, alpha=1 << 30))
         for s, n in zip(seqs, counts):
             self.lengths[s] += n
-        return ids
+        return ids, starts, self.cos[at], self.sin[at]
 
     def _check(self, seqs: list[int], counts: list[int], rows: torch.Tensor) -> None:
         if len(set(seqs)) != len(seqs) or not all(0 <= s < len(self.lengths) for s in seqs):
@@ -88,9 +92,7 @@ class TextTower:
         self._check(seqs, lengths, rows)
         if any(self.lengths[q] for q in seqs):
             raise ValueError("a prompt starts an empty sequence")
-        starts = self._ints([0, *torch.tensor(lengths).cumsum(0).tolist()])
-        cos, sin = self._angles(seqs, lengths)
-        ids = self._grow(seqs, lengths)
+        ids, starts, cos, sin = self._grow(seqs, lengths)
         most, q_dim = max(lengths), s.q_dim
         x = rows.float()
         k = torch.empty(x.shape[0], s.kv_dim, dtype=torch.bfloat16, device=self.dev)
@@ -110,9 +112,8 @@ class TextTower:
         single = counts is None
         counts = [1] * len(seqs) if single else counts
         self._check(seqs, counts, rows)
-        starts = None if single else self._ints([0, *torch.tensor(counts).cumsum(0).tolist()])
-        cos, sin = self._angles(seqs, counts)
-        ids = self._grow(seqs, counts)
+        ids, starts, cos, sin = self._grow(seqs, counts)
+        starts = None if single else starts
         most, q_dim = max(counts), s.q_dim
         x = rows.float()
         for i in range(s.n_layers):
@@ -127,12 +128,12 @@ class TextTower:
         """children[i] (empty) goes on from where parents[i] stands."""
         if len(set(children)) != len(children) or any(self.lengths[c] for c in children):
             raise ValueError("children must be distinct and empty")
-        ops.kv_fork(self.pages, self._ints(parents), self._ints(children))
+        ops.kv_fork(self.pages, *self._put(parents, children))
         for p, c in zip(parents, children):
             self.lengths[c] = self.lengths[p]
 
     def free(self, seqs: list[int]) -> None:
-        ops.kv_free(self.pages, self._ints(seqs))
+        ops.kv_free(self.pages, *self._put(seqs))
         for q in seqs:
             self.lengths[q] = 0
 
@@ -154,7 +155,8 @@ class TextTower:
         """A sequence's cached keys (rotated) and values of one layer, as bf16 rows: what an expert layer that
         cross-attends projects."""
         n = self.lengths[seq]
-        return ops.kv_read(self.pages, layer, self._ints([0, n]), n, self._ints([seq]))
+        starts, ids = self._put([0, n], [seq])
+        return ops.kv_read(self.pages, layer, starts, n, ids)
 
 
 def main() -> None:

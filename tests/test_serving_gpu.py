@@ -210,6 +210,31 @@ def test_tower_goes_on_after_the_pool_ran_out(bundle):  # noqa: F811
         assert off(got[i], plain(bundle, torch.cat([text[q], rows[i : i + 1]]))[-1]) <= TOKEN
 
 
+def test_tower_does_not_wait_for_the_device(bundle):  # noqa: F811
+    """Prompts, tokens, forks, frees and compactions without a copy that the host waits for."""
+    from so101_smolvla_edge_b200.text_tower import TextTower
+
+    tower = TextTower(bundle, n_pages=30, max_seqs=6, max_len=128, page=32)
+    x = torch.randn(60, bundle.spec.text_dim, device="cuda", generator=torch.Generator("cuda").manual_seed(233))
+
+    def turn_of_it():
+        tower.prompt(x[:50], [40, 10], [0, 1])
+        tower.fork([0, 1], [2, 3])
+        tower.step(x[:4], [0, 1, 2, 3])
+        tower.step(x[:9], [1, 3], [4, 5])
+        tower.free([0, 1, 2, 3])
+        tower.compact()
+
+    turn_of_it()  # what the first turn builds
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        turn_of_it()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    tower.check()
+
+
 # ------------------------------------------------------------------------------------------ graphs of attention
 
 
