@@ -72,9 +72,14 @@ class TextTower:
             self.lengths[s] += n
         return ids, starts, self.cos[at], self.sin[at]
 
+    def _check_seqs(self, what: str, seqs: list[int]) -> None:
+        if not all(0 <= s < len(self.lengths) for s in seqs):
+            raise ValueError(f"{what} must be sequences of the cache, 0 to {len(self.lengths) - 1}")
+
     def _check(self, seqs: list[int], counts: list[int], rows: torch.Tensor) -> None:
-        if len(set(seqs)) != len(seqs) or not all(0 <= s < len(self.lengths) for s in seqs):
-            raise ValueError("seqs must be distinct sequences of the cache")
+        self._check_seqs("seqs", seqs)
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("seqs must be distinct")
         if len(counts) != len(seqs) or min(counts, default=1) < 1 or rows.shape != (sum(counts), self.spec.text_dim):
             raise ValueError(f"rows must be ({sum(counts)}, {self.spec.text_dim}), at least one per sequence")
         if any(self.lengths[s] + n > self.pages.max_len for s, n in zip(seqs, counts)):
@@ -90,6 +95,8 @@ class TextTower:
         Returns every row's hidden state (float32)."""
         s = self.spec
         self._check(seqs, lengths, rows)
+        if not seqs:
+            return rows.float()
         if any(self.lengths[q] for q in seqs):
             raise ValueError("a prompt starts an empty sequence")
         ids, starts, cos, sin = self._grow(seqs, lengths)
@@ -112,6 +119,8 @@ class TextTower:
         single = counts is None
         counts = [1] * len(seqs) if single else counts
         self._check(seqs, counts, rows)
+        if not seqs:
+            return rows.float()
         ids, starts, cos, sin = self._grow(seqs, counts)
         starts = None if single else starts
         most, q_dim = max(counts), s.q_dim
@@ -126,13 +135,19 @@ class TextTower:
 
     def fork(self, parents: list[int], children: list[int]) -> None:
         """children[i] (empty) goes on from where parents[i] stands."""
-        if len(set(children)) != len(children) or any(self.lengths[c] for c in children):
-            raise ValueError("children must be distinct and empty")
+        self._check_seqs("parents", parents)
+        self._check_seqs("children", children)
+        if len(parents) != len(children):
+            raise ValueError("there is one parent per child")
+        if len(set(children)) != len(children) or any(self.lengths[c] for c in children) or set(parents) & set(children):
+            raise ValueError("children must be distinct, empty and no parents")
         ops.kv_fork(self.pages, *self._put(parents, children))
         for p, c in zip(parents, children):
             self.lengths[c] = self.lengths[p]
 
     def free(self, seqs: list[int]) -> None:
+        """The sequences give their pages back and are empty."""
+        self._check_seqs("seqs", seqs)
         ops.kv_free(self.pages, *self._put(seqs))
         for q in seqs:
             self.lengths[q] = 0
@@ -154,6 +169,7 @@ class TextTower:
     def cached(self, layer: int, seq: int) -> tuple[torch.Tensor, torch.Tensor]:
         """A sequence's cached keys (rotated) and values of one layer, as bf16 rows: what an expert layer that
         cross-attends projects."""
+        self._check_seqs("seq", [seq])
         n = self.lengths[seq]
         starts, ids = self._put([0, n], [seq])
         return ops.kv_read(self.pages, layer, starts, n, ids)

@@ -235,6 +235,36 @@ def test_tower_does_not_wait_for_the_device(bundle):  # noqa: F811
     tower.check()
 
 
+def test_tower_refuses_what_it_does_not_have(bundle):  # noqa: F811
+    """Numbers outside the cache (negative ones count from the end of a Python list), a child that is a parent too,
+    lists of two lengths; nothing changes. No sequences at all are fine."""
+    from so101_smolvla_edge_b200.text_tower import TextTower
+
+    tower = TextTower(bundle, n_pages=8, max_seqs=4, max_len=64, page=32)
+    x = torch.zeros(5, bundle.spec.text_dim, device="cuda")
+    tower.prompt(x, [5], [3])
+    for call in (
+        lambda: tower.free([-1]),
+        lambda: tower.free([4]),
+        lambda: tower.fork([-1], [0]),
+        lambda: tower.fork([3], [-2]),
+        lambda: tower.fork([3], [4]),
+        lambda: tower.fork([3, 0], [0, 1]),
+        lambda: tower.fork([3], [0, 1]),
+        lambda: tower.cached(0, -1),
+        lambda: tower.step(x[:1], [-1]),
+    ):
+        with pytest.raises(ValueError):
+            call()
+    assert tower.lengths == tower.pages.lengths.tolist() == [0, 0, 0, 5]
+    assert tower.prompt(x[:0], [], []).shape == tower.step(x[:0], []).shape == (0, bundle.spec.text_dim)
+    tower.fork([], [])
+    tower.free([])
+    tower.fork([3], [0])
+    tower.check()
+    assert tower.lengths == tower.pages.lengths.tolist() == [5, 0, 0, 5]
+
+
 # ------------------------------------------------------------------------------------------ graphs of attention
 
 
