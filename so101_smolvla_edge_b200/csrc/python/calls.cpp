@@ -7,8 +7,10 @@
 //
 // Plain CPython functions (METH_FASTCALL): every one takes its arguments by position, raises ValueError for a
 // tensor that the operator does not take, and passes a status other than SO101_OK to the `check` callable that
-// the package registered (its exception types). C++ exceptions become Python ones at the boundary.
+// the package registered (its exception types). C++ exceptions become Python ones at the boundary. The call is made with
+// the tensors' device current: the library launches, looks up and records on the current one.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -273,6 +275,7 @@ PyObject* attention_packed(PyObject* const* a, Py_ssize_t n) {
   int64_t n_starts;
   const int* starts = ints(a[3], "starts", dev, &n_starts);
   const Rope r = rope(a[7], a[8], rows, hd / 2, dev);
+  const c10::cuda::CUDAGuard current(dev);
   const at::Tensor out = result(a[10], rows, heads * hd, dev);
   const Rows ro = bf16_rows(out, "out", rows, heads * hd, dev);
   status(so101_attention_packed(rq.p, rq.ld, rk.p, rk.ld, rv.p, rv.ld, ro.p, ro.ld, rows, starts,
@@ -295,6 +298,7 @@ PyObject* kv_append(PyObject* const* a, Py_ssize_t n) {
   const int* starts = ints(a[4], "starts", dev, &n_starts, true);
   const int* seqs = ints(a[5], "seqs", dev, &n_seqs, true);
   const Rope r = rope(a[7], a[8], rows, c->hd / 2, dev);
+  const c10::cuda::CUDAGuard current(dev);
   status(so101_kv_append(c, small(a[1], "layer"), rk.p, rk.ld, rv.p, rv.ld, rows, starts, seqs,
                          static_cast<int>(entries(n_starts, n_seqs, rows)), integer(a[6]), r.cos, r.sin, stream_of(dev)),
          "so101_kv_append");
@@ -314,6 +318,7 @@ PyObject* kv_read(PyObject* const* a, Py_ssize_t n) {
   const int* first = ints(a[5], "first", dev, &n_first, true);
   const int64_t count = entries(n_starts, n_seqs, rows);
   if (n_first >= 0 && n_first != count) refuse("first has one entry per sequence");
+  const c10::cuda::CUDAGuard current(dev);
   const at::Tensor k = result(Py_None, rows, width, dev), v = result(Py_None, rows, width, dev);
   status(so101_kv_read(c, small(a[1], "layer"), starts, seqs, first, static_cast<int>(count), rows, k.data_ptr(), width,
                        v.data_ptr(), width, stream_of(dev)),
@@ -339,6 +344,7 @@ PyObject* attention_pages(PyObject* const* a, Py_ssize_t n) {
   const int* starts = ints(a[4], "starts", dev, &n_starts, true);
   const int* seqs = ints(a[5], "seqs", dev, &n_seqs, true);
   const Rope r = rope(a[8], a[9], rows, c->hd / 2, dev);
+  const c10::cuda::CUDAGuard current(dev);
   const at::Tensor out = result(a[11], rows, width, dev);
   const Rows ro = bf16_rows(out, "out", rows, width, dev);
   const cudaStream_t stream = stream_of(dev);
@@ -362,6 +368,7 @@ PyObject* lists(PyObject* const* a, Py_ssize_t n, const char* first, const char*
   const int* y = second ? ints(a[2], second, dev, &nb) : nullptr;
   if (second && na != nb) refuse("%s and %s have the same length", first, second);
   if (na > INT32_MAX) refuse("%s is too long", first);
+  const c10::cuda::CUDAGuard current(dev);
   status(call(c, x, y, static_cast<int>(na), stream_of(dev)), name);
   return none();
 }
@@ -383,6 +390,7 @@ PyObject* kv_compact(PyObject* const* a, Py_ssize_t n) {
   need(n, 1);
   c10::Device dev(c10::kCUDA, 0);
   const so101_kv_pages* c = cache(a[0], &dev);
+  const c10::cuda::CUDAGuard current(dev);
   status(so101_kv_compact(c, stream_of(dev)), "so101_kv_compact");
   return none();
 }

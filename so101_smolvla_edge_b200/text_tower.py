@@ -20,6 +20,7 @@ output projection, SwiGLU) under a causal mask; the cache and its sharing have n
 from __future__ import annotations
 
 import argparse
+import functools
 import time
 
 import torch
@@ -30,6 +31,17 @@ from .bundle import Bundle, load_bundle, seeded_bundle
 from .pages import HEAD_DIMS, KvPages
 from .path import Packed, _rope
 from .spec import ModelSpec
+
+
+def _here(method):
+    """A method with its tower's device current, which is where the library launches."""
+
+    @functools.wraps(method)
+    def run(self, *args, **kwargs):
+        with torch.cuda.device(self.dev):
+            return method(self, *args, **kwargs)
+
+    return run
 
 
 class TextTower:
@@ -43,11 +55,12 @@ class TextTower:
         self.dev = torch.device(device)
         if self.dev.index is None:
             self.dev = torch.device("cuda", torch.cuda.current_device())
-        self.packed = Packed.get(self.b, self.dev, (), L.lib())
-        self.w = self.packed.w
-        s = self.spec
-        self.pages = KvPages(s.n_layers, n_pages, s.n_kv, s.head_dim, max_seqs, max_len, page, self.dev)
-        self.cos, self.sin = (t.to(self.dev) for t in _rope(torch.arange(self.pages.max_len), s.head_dim, s.rope_wavelength))
+        with torch.cuda.device(self.dev):
+            self.packed = Packed.get(self.b, self.dev, (), L.lib())
+            self.w = self.packed.w
+            s = self.spec
+            self.pages = KvPages(s.n_layers, n_pages, s.n_kv, s.head_dim, max_seqs, max_len, page, self.dev)
+            self.cos, self.sin = (t.to(self.dev) for t in _rope(torch.arange(self.pages.max_len), s.head_dim, s.rope_wavelength))
         self.lengths = [0] * max_seqs  # the host's own count: what the next positions are
 
     def _put(self, *lists) -> tuple[torch.Tensor, ...]:
@@ -90,6 +103,7 @@ class TextTower:
         h = ops.linear(h, self.w[f"txt.{i}.gate_up"], silu_gate=True)
         return ops.linear(h, self.w[f"txt.{i}.down"], residual=x)
 
+    @_here
     def prompt(self, rows: torch.Tensor, lengths: list[int], seqs: list[int]) -> torch.Tensor:
         """Whole prompts of empty sequences, packed end to end: rows (sum(lengths), text_dim), embedded.
         Returns every row's hidden state (float32)."""
@@ -112,6 +126,7 @@ class TextTower:
             x = self._mlp(i, ops.linear(a, self.w[f"txt.{i}.o"], residual=x))
         return x
 
+    @_here
     def step(self, rows: torch.Tensor, seqs: list[int], counts: list[int] | None = None) -> torch.Tensor:
         """The next tokens of sequences that hold some: one row each, or `counts` (drafted tokens, the rest of a
         prompt). Returns their hidden states (float32)."""
@@ -133,6 +148,7 @@ class TextTower:
             x = self._mlp(i, ops.linear(a, self.w[f"txt.{i}.o"], residual=x))
         return x
 
+    @_here
     def fork(self, parents: list[int], children: list[int]) -> None:
         """children[i] (empty) goes on from where parents[i] stands."""
         self._check_seqs("parents", parents)
@@ -145,6 +161,7 @@ class TextTower:
         for p, c in zip(parents, children):
             self.lengths[c] = self.lengths[p]
 
+    @_here
     def free(self, seqs: list[int]) -> None:
         """The sequences give their pages back and are empty."""
         self._check_seqs("seqs", seqs)
@@ -152,9 +169,11 @@ class TextTower:
         for q in seqs:
             self.lengths[q] = 0
 
+    @_here
     def compact(self) -> None:
         ops.kv_compact(self.pages)
 
+    @_here
     def check(self) -> None:
         """Raise if a call since the last check could not be met (too few free pages). The cache then stands as before
         that call, later calls of its sequences were refused with it (what all of them returned is void), and this
@@ -166,6 +185,7 @@ class TextTower:
             self.lengths = self.pages.lengths.tolist()
             L.check(status, "TextTower")
 
+    @_here
     def cached(self, layer: int, seq: int) -> tuple[torch.Tensor, torch.Tensor]:
         """A sequence's cached keys (rotated) and values of one layer, as bf16 rows: what an expert layer that
         cross-attends projects."""

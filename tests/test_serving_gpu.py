@@ -265,6 +265,24 @@ def test_tower_refuses_what_it_does_not_have(bundle):  # noqa: F811
     assert tower.lengths == tower.pages.lengths.tolist() == [5, 0, 0, 5]
 
 
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_of_another_device_than_the_current_one(bundle):  # noqa: F811
+    from so101_smolvla_edge_b200.text_tower import TextTower
+
+    x = torch.randn(9, bundle.spec.text_dim, generator=torch.Generator().manual_seed(235))
+    got = []
+    for dev in ("cuda:0", "cuda:1"):  # the first is current throughout
+        tower = TextTower(bundle, n_pages=8, max_seqs=2, max_len=64, page=32, device=dev)
+        rows = x.to(dev)
+        out = [tower.prompt(rows[:7], [7], [0])]
+        tower.fork([0], [1])
+        out.append(tower.step(rows[7:], [0, 1]))
+        tower.compact()
+        tower.check()
+        got.append([y.cpu() for y in (*out, *tower.cached(1, 0))])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 # ------------------------------------------------------------------------------------------ graphs of attention
 
 
