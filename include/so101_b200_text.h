@@ -25,7 +25,8 @@ extern "C" {
  * [h*hd, (h+1)*hd); k, v: (rows, >= nkv*hd). Sequence i is rows [starts[i], starts[i+1]) of all
  * three (starts: n_seqs + 1 int32, non-decreasing, starts[n_seqs] <= rows; empty sequences are
  * fine); its row r sees its rows 0..r and nothing else, whatever the other rows hold (infinities
- * and NaN included). max_len: at least the longest sequence. cos / sin (rows, hd/2 fp32) rotate q
+ * and NaN included). max_len: 0 where all of them are empty (nothing is launched); else without
+ * effect, the lengths are read from starts. cos / sin (rows, hd/2 fp32) rotate q
  * on load in fp32 (NULL: none), kept as two bf16 parts; k comes rotated. scale multiplies q.k. hd 64
  * or 128; 16-byte aligned bases (cos and sin too) and row strides. Rows outside every sequence are
  * not written. */
@@ -85,7 +86,8 @@ SO101_API int so101_kv_read(const so101_kv_pages* c, int layer, const int* start
  * sin are 16-byte aligned, o 8-byte; ldq is a multiple of 8, ldo of 4. Probabilities
  * are rounded to fp16, sums are fp32. workspace (fp32 partials) and tickets (zero before the first
  * call, left zero) join the parts of a sequence that several CTAs read: 40 MB and 1184 tickets let every
- * shape use the whole GPU, with less it uses fewer CTAs. */
+ * shape use the whole GPU, with less it uses fewer CTAs. Calls that may run at the same time (other
+ * streams, other graphs) need a workspace and tickets each; after SO101_ERR_TIMEOUT zero the tickets. */
 SO101_API int so101_attention_pages(const void* q, int64_t ldq, void* o, int64_t ldo, int64_t rows,
                                     const so101_kv_pages* c, int layer, int nq, const int* starts,
                                     const int* seqs, int n_seqs, int64_t max_q, int causal, float scale,

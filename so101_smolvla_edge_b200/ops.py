@@ -516,7 +516,7 @@ def attention_packed(
 
     q is (rows, n_heads * hd), k and v (rows, n_kv * hd), bf16 with any row stride (slices of the
     fused qkv rows), head_dim 64 or 128. Sequence i is rows starts[i]:starts[i + 1] (int32, on the
-    device); its row r sees its rows 0..r only, whatever the others hold. max_len is at least the longest sequence. cos
+    device); its row r sees its rows 0..r only, whatever the others hold. max_len: 0 where all are empty, else without effect. cos
     and sin (rows, hd / 2) rotate q; k comes rotated (`rope_kv`). scale defaults to hd ** -0.5.
     Rows outside every sequence are left as they are.
     """

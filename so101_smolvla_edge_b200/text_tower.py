@@ -14,7 +14,10 @@ continuations or noise samples of one observation) and give their memory back:
     tower.free([2, 3]); tower.compact()
 
 The layers are the reference's prefix layers (pkg/model/smolvla_triton.py:78-103: RMSNorm, fused q|k|v, RoPE, attention,
-output projection, SwiGLU) under a causal mask; the cache and its sharing have no counterpart there.
+output projection, SwiGLU), but under a causal mask, as a language model runs them; in the policy's prefix images
+and task tokens see each other. From the second layer on the hidden states, keys and values are therefore not those
+that the policy's action expert was trained on: its chunks come from `Engine`. A bundle holds neither a token embedding nor an output
+head, so rows come in embedded and go out as hidden states. The cache and its sharing have no counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -187,8 +190,7 @@ class TextTower:
 
     @_here
     def cached(self, layer: int, seq: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """A sequence's cached keys (rotated) and values of one layer, as bf16 rows: what an expert layer that
-        cross-attends projects."""
+        """A sequence's cached keys (rotated) and values of one layer, as bf16 rows (of a causal pass: see the top)."""
         self._check_seqs("seq", [seq])
         n = self.lengths[seq]
         starts, ids = self._put([0, n], [seq])
