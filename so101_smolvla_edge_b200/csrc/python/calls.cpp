@@ -173,8 +173,9 @@ struct Held {
   CaptureKey key;
 };
 std::map<CaptureKey, Space> g_captured;  // under the interpreter lock, as g_spaces
-std::mutex g_ended_lock;
-std::vector<Held*> g_ended;
+// (never destroyed: the driver may end the last graphs after this module's own objects are gone)
+std::mutex& g_ended_lock = *new std::mutex;
+std::vector<Held*>& g_ended = *new std::vector<Held*>;
 
 void CUDART_CB graph_ended(void* held) {
   const std::lock_guard<std::mutex> lock(g_ended_lock);

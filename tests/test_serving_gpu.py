@@ -374,3 +374,23 @@ def test_a_graphs_workspace_goes_with_it():
             break
         time.sleep(0.02)
     assert torch.cuda.memory_allocated() <= before
+
+
+def test_a_graph_outlives_the_program():
+    """A process that ends with a graph alive ends well."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import sys
+sys.path[:0] = ['.', 'tests']
+from test_serving_gpu import attention_graphs
+import builtins, torch
+builtins.kept = attention_graphs(2)
+[g.replay() for g, *_ in builtins.kept]
+torch.cuda.synchronize()
+"""
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr
