@@ -470,6 +470,18 @@ def device_status() -> int:
     return L.lib().so101_device_status()
 
 
+def clear_device_status() -> None:
+    """Clear the status word. A call of `attention_pages` whose waits ran out (ERR_TIMEOUT) may leave tickets counted, by which
+    later calls would join too early or never: those of every stream of the device are cleared with it. Waits for the device."""
+    torch.cuda.synchronize()
+    if device_status() == L.ERR_TIMEOUT:
+        for (device, _), ws in list(_PAGES_WS.items()):
+            if device == torch.cuda.current_device():
+                ws.tickets.zero_()
+        torch.cuda.synchronize()
+    L.check(L.lib().so101_clear_device_status(), "so101_clear_device_status")
+
+
 def set_pdl(enable: bool) -> None:
     """Launch GEMMs with programmatic dependent launch (they start streaming weights while the
     previous kernel on the stream drains)."""

@@ -184,7 +184,7 @@ class TextTower:
         torch.cuda.current_stream(self.dev).synchronize()
         status = ops.device_status()
         if status != L.OK:
-            L.lib().so101_clear_device_status()
+            ops.clear_device_status()
             self.lengths = self.pages.lengths.tolist()
             L.check(status, "TextTower")
 

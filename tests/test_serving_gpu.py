@@ -283,6 +283,23 @@ def test_tensors_of_another_device_than_the_current_one(bundle):  # noqa: F811
     assert all(torch.equal(a, b) for a, b in zip(*got))
 
 
+def test_tickets_after_a_wait_that_ran_out(monkeypatch):
+    """What a call that gave up leaves behind (tickets counted in part, put there by hand) goes with the status."""
+    from so101_smolvla_edge_b200 import _lib as L
+    from so101_smolvla_edge_b200 import ops
+
+    c = cache([9000, 5000], 2, 64, 64, seed=237)
+    q = queries(2, 6, 64, seed=238)
+    want = ops.attention_pages(q, c, 0, 6)
+    stream = torch.cuda.current_stream()
+    ops.pages_workspace(stream.device.index, stream.cuda_stream).tickets.fill_(1)
+    with monkeypatch.context() as m:
+        m.setattr(ops, "device_status", lambda: L.ERR_TIMEOUT)
+        ops.clear_device_status()
+    assert ops.device_status() == 0
+    assert torch.equal(ops.attention_pages(q, c, 0, 6), want)
+
+
 # ------------------------------------------------------------------------------------------ graphs of attention
 
 
