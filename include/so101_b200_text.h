@@ -59,7 +59,7 @@ SO101_API int so101_kv_scratch(const so101_kv_pages* c, int64_t* ints);
 
 /* Quantise new tokens into the pages of one layer. k, v: (rows, >= n_kv*hd) bf16, rows
  * [starts[i], starts[i+1]) being the LAST tokens of sequence seqs[i] (lengths already count them:
- * so101_kv_reserve; starts NULL: one row per sequence; seqs NULL: sequence i). max_new: at least
+ * so101_kv_reserve; starts NULL: one row per sequence; seqs NULL: sequence i), which are distinct. max_new: at least
  * the most rows of a sequence. cos / sin (rows, hd/2 fp32) rotate the keys first, in fp32, as
  * so101_rope_kv does but without its rounding to bf16 (NULL: none). k, v, cos, sin 16-byte aligned, ldk and
  * ldv multiples of 8. The rule, per page and head:

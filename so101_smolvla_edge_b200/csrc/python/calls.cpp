@@ -89,7 +89,7 @@ Rows bf16_rows(const at::Tensor& t, const char* name, int64_t rows, int64_t cols
     refuse("%s must be bf16 (%lld, %lld) on %s", name, static_cast<long long>(rows), static_cast<long long>(cols),
            dev.str().c_str());
   if (t.stride(1) != 1 && cols > 1) refuse("%s needs unit column stride", name);
-  return {t.data_ptr(), t.stride(0)};
+  return {t.data_ptr(), rows > 1 ? t.stride(0) : cols};  // (a single row's stride may be anything)
 }
 
 // A contiguous int32 vector, or null where None is allowed.

@@ -411,3 +411,16 @@ torch.cuda.synchronize()
     root = Path(__file__).resolve().parents[1]
     done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
     assert done.returncode == 0, done.stderr
+
+
+def test_a_single_row_of_any_stride():
+    """A row whose stride says nothing (a transposed column) is a row like another."""
+    from so101_smolvla_edge_b200 import ops
+
+    c, d = (cache([70], 2, 64, 64, seed=281) for _ in range(2))
+    for one, two in ((lambda t: t, c), (lambda t: t.reshape(-1, 1).clone().t(), d)):
+        g = torch.Generator("cuda").manual_seed(282)
+        q, k, v = (one(torch.randn(1, n, device="cuda", generator=g).to(torch.bfloat16)) for n in (384, 128, 128))
+        ops.kv_append(two, 0, k, v)
+        two.got = (ops.attention_pages(q, two, 0, 6), ops.attention_packed(q, k, v, ints([0, 1]), 1, 6, 2))
+    assert d.k.equal(c.k) and all(torch.equal(a, b) for a, b in zip(c.got, d.got))
